@@ -236,7 +236,8 @@ def _adamw_out(s):
 
 def _int8(s):
     x = s["x"].float()
-    sx = x.abs().amax(1) / 127
+    amax = x.abs().amax(1)
+    sx = amax / torch.full_like(amax, 127)                 # (by a number it would be a product with 1 / 127)
     # 64 bits for the quotient: a value next to the middle of two integers goes to the nearer one
     q = torch.round(x.double() / sx.double()[:, None].clamp_min(1e-300)).clamp_(-127, 127).float()
     y = (q @ s["wq"].float().t()) * sx[:, None] * s["ws"]
@@ -371,7 +372,7 @@ def exact(case, seed):
                 out[k].append(got[k])
         return out
     x = s["x"].to(f)
-    sx = (x.abs().amax(1).float() / 127).to(f)              # the scale is held in 32 bits
+    sx = (x.abs().amax(1) / 127).float().to(f)              # the scale is held in 32 bits
     q = torch.round(x / torch.where(sx > 0, sx, torch.ones_like(sx))[:, None]).clamp(-127, 127)
     y = torch.mm(q, s["wq"].to(f).t().contiguous()) * (sx[:, None] * s["ws"].to(f)[None, :])
     return y if s["bias"] is None else y + s["bias"].to(f)
