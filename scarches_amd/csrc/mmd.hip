@@ -131,11 +131,11 @@ __global__ __launch_bounds__(256) void mmd_prepare_kernel(const int32_t* __restr
 // K = sum_a exp(-beta_a d2), Kp = sum_a beta_a exp(-beta_a d2) over the 19 bandwidths: three exps + one polynomial
 // pair in the common case - see rbf19 below.
 typedef float v2f __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ v2f pk_fma(v2f a, v2f b, v2f c) { return __builtin_elementwise_fma(a, b, c); }   // v_pk_fma_f32
+__device__ __forceinline__ v2f pk_fma(v2f a, v2f b, v2f c) { return __builtin_elementwise_fma(a, b, c); }
 
-// KK[u] = (K, Kp) of pair u.  Written for the packed fp32 VALU ops of gfx950 (two lanes of work per instruction):
-// the exp arguments of two pairs share one v_pk_mul_f32, each exp feeds (K, Kp) with one v_pk_fma_f32, and the two
-// Horner chains of the polynomial pair (rbf19) run as one packed chain.
+// KK[u] = (K, Kp) of pair u.  Written in pairs: the exp arguments of two pairs are scaled together, each exp feeds
+// (K, Kp), and the two Horner chains of the polynomial pair (rbf19) run side by side.  (Two fp32 instructions per pair:
+// the build keeps packed fp32 off, see the Makefile.)
 template <int U>
 __device__ __forceinline__ void rbf_terms(int a, const float (&d2)[U], v2f (&KK)[U]) {
     constexpr float LOG2E = 1.4426950408889634f;
