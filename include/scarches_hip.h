@@ -329,6 +329,73 @@ int sca_bn_bwd(const float* dh, int S, long long slab_stride, const float* extra
                const uint8_t* mask, uint64_t seed, uint32_t rng_stream, const uint32_t* step, double* acc, float* da,
                float* dgamma, float* dbeta, void* stream);
 
+/* ---- layer norm with weight and bias -----------------------------------------------------------------------------
+ * h = (x - mean) * rstd over each row's n values, rstd = 1 / sqrt(var + eps) (biased variance), y = h * w + b, and its
+ * backward pass with the reduction over rows of the weight's and the bias' gradient.  (The layers of the conditional
+ * networks normalise without weight and bias inside sca_layer_fwd / sca_layer_bwd; nn.LayerNorm(elementwise_affine=True)
+ * is what these two replace.)
+ * dtype of x, y, dy, dx: 0 fp32, 1 bf16, 2 fp16; wtype of w, b, dw, db: 0 or dtype.  Rows of pitch ld* elements (>= n for
+ * outputs; any pitch from 0 - one row read again and again - for inputs), any alignment.  w / b may be NULL (1 / 0).
+ * stats [2][rows] = (mean, rstd), fp32; may be NULL in the forward pass.  Sums and statistics are held in fp32, each
+ * result is rounded once.  sca_layernorm_bwd: dx, dw, db may each be NULL; ws: scratch of
+ * sca_layernorm_bwd_workspace_floats(rows, n) floats, only for dw / db (any contents on entry; a workspace must not be
+ * shared by calls that may overlap).  Sums over rows are taken in a fixed order: the same call gives the same bits.
+ * rows = 0: nothing is read, dw and db become 0.  -1 for an argument outside these ranges. */
+int sca_layernorm_fwd(const void* x, long long ldx, int dtype, long long rows, int n, const void* w, const void* b,
+                      int wtype, float eps, void* y, long long ldy, float* stats, void* stream);
+long long sca_layernorm_bwd_workspace_floats(long long rows, int n);
+int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, int dtype, long long rows, int n,
+                      const void* w, int wtype, const float* stats, void* dx, long long lddx, void* dw, void* db,
+                      float* ws, void* stream);
+
+/* ---- AdamW over a list of tensors ----------------------------------------------------------------------------------
+ * m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ * p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * for every tensor of a table in ONE launch (torch.optim.AdamW; sca_adam_step is the coupled form on one range).
+ * `tensors` and `chunks` lie in DEVICE memory: one sca_adamw_tensor per tensor, and for tensor j the entries {j, 0}, {j, 1},
+ * ... of ceil(n / sca_adamw_chunk_elements()) chunks.  p and g: dtype 0 fp32, 1 bf16, 2 fp16 (computed in fp32, rounded
+ * once).  vec = 1 promises that p, g and - with 32-bit states - m, v are aligned to 4 of their elements, and with 8-bit
+ * states m, v to 4 bytes; 0 makes no such promise.
+ * state_bits 32: m, v fp32 [n].  state_bits 8: m e4m3 bytes [n], v e5m2 bytes [n] (the OCP types), each standing for
+ * value * scale with one fp32 power of two per sca_adamw_block_elements() consecutive elements in m_scale / v_scale;
+ * rounding is stochastic: the 16 low (m) / high (v) bits of word i & 3 of Philox4x32-10(counter (i >> 2, id, t), key seed)
+ * decide for element i (common.h's generator).  A block with a value that is not finite keeps scale NaN.
+ * Step number: hyper != NULL (32-bit states only) reads lr, the bias corrections, eps and the clip value from the block that
+ * sca_begin_step fills; hyper = NULL uses lr / eps as given, t = *step + 1 per tensor, and the launch advances every *step
+ * of the table by 1 at its end.  done: one uint32, 0 before the first launch and left 0 by each (hyper = NULL); steps, done
+ * and the tensors belong to one launch at a time.  No tensor may appear twice in a table. */
+typedef struct {
+    void* p; const void* g; void* m; void* v;
+    float* m_scale; float* v_scale;
+    long long n;
+    int64_t* step;
+    float weight_decay;
+    int32_t dtype, vec, id;
+} sca_adamw_tensor;
+typedef struct {
+    int32_t tensor, index;
+} sca_adamw_chunk;
+int sca_adamw_chunk_elements(void);
+int sca_adamw_block_elements(void);
+int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_adamw_chunk* chunks, int n_chunks,
+                   int state_bits, const float* hyper, float lr, double beta1, double beta2, float eps, uint64_t seed,
+                   uint32_t* done, void* stream);
+
+/* ---- product in 8-bit integers -------------------------------------------------------------------------------------
+ * sca_quant_rows_i8: scale[r] = max_k |x_rk| / 127, q_rk = round(x_rk / scale[r]) (ties to even, the exact quotient), and
+ * q_rk = 0 for k <= column < ldq.  x: dtype 0 fp32, 1 bf16, 2 fp16, rows of pitch ldx.  A row of zeros has scale 0; a row
+ * with a value that is not finite has scale NaN and q = 0, so that what is computed from it is NaN.
+ * sca_gemm_i8: y[m][n] = (sum_k xq[m][k] wq[n][k]) * sx[m] * sw[n] + bias[n], the sum exact in int32 (K <=
+ * sca_gemm_i8_max_k()), the rest in fp32, rounded once to ytype.  wq is a torch Linear weight [N][K] in int8 with pitch ldw.
+ * bias (may be NULL): btype 0 or ytype.  Any pitches and alignments; 16-byte aligned operands whose pitch is a multiple of
+ * 16 take the faster loads.  The forward product y = x W^T of the reference's nn.Linear layers
+ * (scarches/models/trvae/modules.py:21-27) for serving. */
+int sca_gemm_i8_max_k(void);
+int sca_quant_rows_i8(const void* x, long long ldx, int dtype, long long rows, int k, int8_t* q, long long ldq,
+                      float* scale, void* stream);
+int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, const int8_t* wq, long long ldw, const float* sw,
+                const void* bias, int btype, long long M, int N, int K, void* y, int ytype, long long ldy, void* stream);
+
 /* ---- expiMap ---------------------------------------------------------------------------------------------------
  * sca_masked_copy: dst[r*ldd+c] = src[r*lds+c] * (mask ? mask[r*ldm+c] : 1).  Packs MaskedLinear weights
  * (weight*mask, models/expimap/modules.py:24-25) of expr_L / ext_L_m / ext_L into ONE decoder matrix

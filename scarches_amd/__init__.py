@@ -11,5 +11,5 @@ fallback: importing works anywhere, using a model needs a gfx950 device and the 
 """
 __version__ = "0.1.0"
 
-from . import dataset, models, trainers, utils  # noqa: E402,F401
+from . import dataset, models, ops, trainers, utils  # noqa: E402,F401
 from .anndata_lite import CellData  # noqa: E402,F401

@@ -16,6 +16,7 @@ P = C.c_void_p
 I = C.c_int
 LL = C.c_longlong
 F = C.c_float
+D = C.c_double
 U64 = C.c_uint64
 U32 = C.c_uint32
 
@@ -53,6 +54,13 @@ class MidArgs(C.Structure):
                 ("dheads", C.c_void_p), ("dh_out", C.c_void_p),
                 ("fuse_first", C.c_int32), ("S0", C.c_int32), ("pre0", C.c_void_p), ("pre0_stride", C.c_longlong),
                 ("first", MidLayer)]
+
+
+class AdamWTensor(C.Structure):
+    """sca_adamw_tensor of include/scarches_hip.h."""
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n", C.c_longlong), ("step", C.c_void_p),
+                ("weight_decay", C.c_float), ("dtype", C.c_int32), ("vec", C.c_int32), ("id", C.c_int32)]
 
 
 # name -> argtypes (restype is always int); mirrors include/scarches_hip.h one to one
@@ -137,6 +145,15 @@ SIGNATURES = {
     "sca_grad_tail": [P, I, P],
     "sca_bn_fwd": [P, I, I, P, P, P, P, I, I, F, F, P, U64, U32, P, P, P, P, P],
     "sca_bn_bwd": [P, I, LL, P, I, I, P, P, P, P, I, F, P, U64, U32, P, P, P, P, P, P],
+    "sca_layernorm_fwd": [P, LL, I, LL, I, P, P, I, F, P, LL, P, P],
+    "sca_layernorm_bwd_workspace_floats": [LL, I],
+    "sca_layernorm_bwd": [P, LL, P, LL, I, LL, I, P, I, P, P, LL, P, P, P, P],
+    "sca_adamw_chunk_elements": [],
+    "sca_adamw_block_elements": [],
+    "sca_adamw_step": [P, I, P, I, I, P, F, D, D, F, U64, P, P],
+    "sca_gemm_i8_max_k": [],
+    "sca_quant_rows_i8": [P, LL, I, LL, I, P, LL, P, P],
+    "sca_gemm_i8": [P, LL, P, P, LL, P, P, I, LL, I, I, P, I, LL, P],
     "sca_embed_lookup": [P, I, I, P, I, I, F, P, P, I, P],
     "sca_embed_scatter_add": [P, P, I, I, I, I, P, I, P, P],
     "sca_proto_workspace_bytes": [I, I, I],
@@ -145,7 +162,8 @@ SIGNATURES = {
     "sca_class_moments": [P, I, I, I, P, I, P, I, P, P, P, P],
     "sca_class_moments_finish": [P, P, P, I, I, P, P, P, P, P, P],
 }
-RESTYPES = {"sca_hsic_workspace_floats": LL, "sca_proto_workspace_bytes": LL, "sca_knn_static_max_entries": LL}
+RESTYPES = {"sca_hsic_workspace_floats": LL, "sca_proto_workspace_bytes": LL, "sca_knn_static_max_entries": LL,
+            "sca_layernorm_bwd_workspace_floats": LL}
 
 _lib = None
 ABI_VERSION = 3       # sca_abi_version() of the library this binding was written against

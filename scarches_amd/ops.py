@@ -1,0 +1,464 @@
+"""Operators around the dense layers of a network, on tensors of a HIP device: layer norm with weight and bias (forward,
+backward, autograd), AdamW over a network's whole parameter list (32-bit or 8-bit states), and the product in 8-bit integers
+with a scale per row and per output channel for serving.
+
+    y = ops.layer_norm(x, weight, bias)                          # differentiable
+    opt = ops.AdamW(net.parameters(), lr=1e-3, state_bits=8)     # torch.optim.Optimizer
+    wq, ws = ops.quantize_int8(weight)                           # once
+    y = ops.int8_linear(x, wq, ws, bias)                         # per request
+
+All arithmetic runs in the HIP kernels behind include/scarches_hip.h (sca_layernorm_*, sca_adamw_step, sca_quant_rows_i8,
+sca_gemm_i8) on the current stream of the tensors' device; there is no CPU fallback.  Wrong shapes and types raise ValueError
+/ TypeError before anything is launched.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import numpy as np
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F8_M, _F8_V = torch.float8_e4m3fn, torch.float8_e5m2
+
+
+def _dtype_code(t: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the operator's other tensors on {device}")
+    if device.type != "cuda":
+        raise _lib.HipLibraryError("scarches_amd runs on a HIP device only (no CPU fallback)")
+
+
+def _call(device, name, *args):
+    """One entry point of the library on `device`, behind what its current stream holds."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+def _rows(t: torch.Tensor):
+    """(tensor whose rows are contiguous, rows, pitch) of a [..., n] tensor; a copy only where no such view exists."""
+    n = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, n)
+    if n > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    rows = t.shape[0]
+    return t, rows, t.stride(0) if rows > 1 else n
+
+
+# ---------------------------------------------------------------------------------------------- layer norm
+def _ln_check(x, weight, bias):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"layer norm needs a last dimension of at least one value, got shape {tuple(x.shape)}")
+    code = _dtype_code(x, "x")
+    if weight is None:
+        if bias is not None:
+            raise ValueError("layer norm takes a bias only together with a weight")
+        return code, code
+    n = x.shape[-1]
+    wcode = _dtype_code(weight, "weight")
+    if wcode not in (0, code):
+        raise TypeError(f"weight must be float32 or of x's type {x.dtype}, not {weight.dtype}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (n,):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, x's rows need ({n},)")
+        if t.dtype != weight.dtype:
+            raise TypeError(f"weight is {weight.dtype}, bias {t.dtype}")
+        if t.stride(0) != 1 and n > 1:
+            raise ValueError(f"{name} must be contiguous")
+    return code, wcode
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
+    """(y, stats): layer norm of the rows of x [..., n] (float32, bfloat16 or float16, rows of any pitch) and stats [2, rows]
+    = (mean, 1 / sqrt(variance + eps)) in float32 for `layer_norm_bwd`.  weight / bias: [n], float32 or x's type."""
+    code, wcode = _ln_check(x, weight, bias)
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    dev = x.device
+    _same_device(dev, weight=weight, bias=bias)
+    x2, rows, ldx = _rows(x)
+    n = x.shape[-1]
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    if rows:
+        _call(dev, "sca_layernorm_fwd", x2.data_ptr(), ldx, code, rows, n, _lib.ptr(weight), _lib.ptr(bias), wcode,
+              float(eps), y.data_ptr(), n, stats.data_ptr())
+    return y, stats
+
+
+def layer_norm_bwd(dy, x, weight, stats, need=(True, True, True)):
+    """(dx, dweight, dbias) of layer norm for the gradient dy of its result: x and weight as they were given to
+    `layer_norm_fwd`, stats as it returned them.  `need`: which of the three are wanted (the others are None, and so are
+    dweight and dbias without a weight).  dweight and dbias are sums over all rows, taken in float32 in a fixed order."""
+    code, wcode = _ln_check(x, weight, None)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy is {dy.dtype} {tuple(dy.shape)}, x {x.dtype} {tuple(x.shape)}")
+    dev = x.device
+    _same_device(dev, dy=dy, weight=weight, stats=stats)
+    x2, rows, ldx = _rows(x)
+    dy2, _, lddy = _rows(dy)
+    n = x.shape[-1]
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
+        raise ValueError(f"stats must be the float32 tensor [2, {rows}] that the forward pass returned")
+    need_w, need_b = need[1] and weight is not None, need[2] and weight is not None
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+    dw = torch.empty(n, dtype=weight.dtype, device=dev) if need_w else None
+    db = torch.empty(n, dtype=weight.dtype, device=dev) if need_b else None
+    ws = None
+    if need_w or need_b:
+        ws = torch.empty(_lib.load().sca_layernorm_bwd_workspace_floats(rows, n), dtype=torch.float32, device=dev)
+    _call(dev, "sca_layernorm_bwd", dy2.data_ptr(), lddy, x2.data_ptr(), ldx, code, rows, n, _lib.ptr(weight), wcode,
+          stats.data_ptr(), _lib.ptr(dx), n, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws))
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, stats)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        return (*layer_norm_bwd(dy, x, weight, stats, ctx.needs_input_grad[:3]), None)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last dimension of x with optional weight and bias [n]; gradients of x, weight and bias.
+
+    Statistics and sums are held in float32 whatever x's type, and each result is rounded once.  A row with NaN or an
+    infinity gives NaN in that row (and in the weight's gradient) only."""
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return layer_norm_fwd(x, weight, bias, eps)[0]
+
+
+# ---------------------------------------------------------------------------------------------- 8-bit integer product
+_PAD_K = 128        # pitch of quantized rows: a multiple of the product's k step, the bytes behind a row's end are zero
+
+
+def quantize_int8(x):
+    """(q, scale) of the rows of x [..., k]: int8 q [..., k] and float32 scale [...] with x ~ q * scale[..., None], scale =
+    max |x| / 127 of the row.  q is a view of rows padded with zeros to a multiple of 128 bytes, as `int8_matmul` reads them
+    fastest.  A row of zeros has scale 0; a row with NaN or an infinity has scale NaN, and so have results computed from it."""
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"quantize_int8 needs rows of at least one value, got shape {tuple(x.shape)}")
+    code = _dtype_code(x, "x")
+    _same_device(x.device)
+    x2, rows, ldx = _rows(x)
+    k = x.shape[-1]
+    pitch = -(-k // _PAD_K) * _PAD_K
+    q = torch.empty((*x.shape[:-1], pitch), dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if rows:
+        _call(x.device, "sca_quant_rows_i8", x2.data_ptr(), ldx, code, rows, k, q.data_ptr(), pitch, scale.data_ptr())
+    return q[..., :k], scale
+
+
+def _i8_check(k, wq, w_scale, bias, out_dtype):
+    if out_dtype not in _DTYPES:
+        raise TypeError(f"results can be float32, bfloat16 or float16, not {out_dtype}")
+    if wq.dtype != torch.int8 or wq.dim() != 2:
+        raise TypeError(f"wq must be an int8 matrix [out, in], not {wq.dtype} {tuple(wq.shape)}")
+    n = wq.shape[0]
+    if wq.shape[1] != k or k == 0:
+        raise ValueError(f"x has rows of {k} values, wq is {tuple(wq.shape)}")
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (n,) or (n > 1 and w_scale.stride(0) != 1):
+        raise ValueError(f"w_scale must be a contiguous float32 vector [{n}], one value per output channel")
+    if bias is not None and (tuple(bias.shape) != (n,) or bias.dtype not in (torch.float32, out_dtype)
+                             or (n > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"bias must be a contiguous vector [{n}] of float32 or {out_dtype}")
+    if k > _lib.load().sca_gemm_i8_max_k():
+        raise ValueError(f"rows of {k} values: the sum of more than {_lib.load().sca_gemm_i8_max_k()} products can pass int32")
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the 8-bit integer product is for serving and has no gradient: call it under torch.no_grad()")
+
+
+def _i8_product(xq_ptr, ldx, sx_ptr, wq, w_scale, bias, shape, rows, k, out_dtype):
+    n = wq.shape[0]
+    y = torch.empty((*shape, n), dtype=out_dtype, device=wq.device)
+    if rows and n:
+        if k > 1 and wq.stride(1) != 1:
+            wq = wq.contiguous()
+        _call(wq.device, "sca_gemm_i8", xq_ptr, ldx, sx_ptr, wq.data_ptr(), wq.stride(0) if n > 1 else k, w_scale.data_ptr(),
+              _lib.ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], rows, n, k, y.data_ptr(),
+              _DTYPES[out_dtype], n)
+    return y
+
+
+def int8_matmul(xq, x_scale, wq, w_scale, bias: Optional[torch.Tensor] = None, out_dtype=torch.float32):
+    """y [..., n] = (xq wq^T) * x_scale[..., None] * w_scale + bias for int8 xq [..., k] with one scale per row (as
+    `quantize_int8` gives them) and an int8 weight wq [n, k] with one scale per output channel.  The integer sum is exact
+    (k < 2^17); scales and bias are applied in float32 and the result is rounded once to out_dtype."""
+    if xq.dtype != torch.int8 or xq.dim() < 1:
+        raise TypeError(f"xq must be int8 rows [..., k], not {xq.dtype} {tuple(xq.shape)}")
+    k = xq.shape[-1]
+    _i8_check(k, wq, w_scale, bias, out_dtype)
+    if x_scale.dtype != torch.float32 or x_scale.shape != xq.shape[:-1] or not x_scale.is_contiguous():
+        raise ValueError(f"x_scale must be contiguous float32 {tuple(xq.shape[:-1])}, one value per row of xq")
+    _no_grad(x_scale, w_scale, bias)
+    _same_device(wq.device, xq=xq, x_scale=x_scale, w_scale=w_scale, bias=bias)
+    x2, rows, ldx = _rows(xq)
+    return _i8_product(x2.data_ptr(), ldx, x_scale.data_ptr(), wq, w_scale, bias, xq.shape[:-1], rows, k, out_dtype)
+
+
+def int8_linear(x, wq, w_scale, bias: Optional[torch.Tensor] = None, out_dtype=None):
+    """y = x W^T + bias in 8-bit integers: x [..., k] (float32, bfloat16 or float16) is quantized row by row as by
+    `quantize_int8`, then multiplied as by `int8_matmul`.  out_dtype: x's type by default.  Serving only: no gradient."""
+    if x.dim() < 1:
+        raise ValueError("int8_linear needs rows [..., k]")
+    code = _dtype_code(x, "x")
+    k = x.shape[-1]
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _i8_check(k, wq, w_scale, bias, out_dtype)
+    _no_grad(x, w_scale, bias)
+    dev = x.device
+    _same_device(dev, wq=wq, w_scale=w_scale, bias=bias)
+    x2, rows, ldx = _rows(x)
+    pitch = -(-k // _PAD_K) * _PAD_K
+    buf = torch.empty(rows * (pitch + 4), dtype=torch.int8, device=dev)    # the quantized rows, then their scales
+    q_ptr, scale_ptr = buf.data_ptr(), buf.data_ptr() + rows * pitch
+    if rows:
+        _call(dev, "sca_quant_rows_i8", x2.data_ptr(), ldx, code, rows, k, q_ptr, pitch, scale_ptr)
+    return _i8_product(q_ptr, pitch, scale_ptr, wq, w_scale, bias, x.shape[:-1], rows, k, out_dtype)
+
+
+# ---------------------------------------------------------------------------------------------- AdamW
+def _layout(t):
+    """What two tensors have in common whose elements lie in the same order: () if contiguous, else the strides."""
+    return () if t.is_contiguous() else tuple(t.stride())
+
+
+def _dense(t):
+    """True when t's elements fill one range of memory, each once (any order of the dimensions)."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for stride, n in sorted((t.stride(d), t.shape[d]) for d in range(t.dim()) if t.shape[d] != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW (decoupled weight decay) over all parameters of a group in one launch.
+
+    params, lr, betas, eps, weight_decay: as torch.optim.AdamW.  Parameters are float32, bfloat16 or float16; a step is
+    computed in float32 and rounded once.
+    state_bits=32: `exp_avg`, `exp_avg_sq` in float32 whatever the parameter's type.
+    state_bits=8: `exp_avg` float8_e4m3fn and `exp_avg_sq` float8_e5m2, each with one float32 power of two per 256 elements
+    (`exp_avg_scale`, `exp_avg_sq_scale`): 2.03 bytes per value instead of 8.  Rounding to 8 bits is stochastic, from a
+    generator of (seed, parameter, element, step): the same seed gives the same run.  A gradient that is not finite makes
+    the moments of its 256 elements NaN.
+
+    The step number of each parameter lies on the device, so `step()` may be captured into a HIP graph after one ordinary
+    call with the same gradients' storage (lr and the other scalars are taken as they are at capture; a graph captured before
+    `load_state_dict` goes on with the states it was captured with).  Gradients have their parameter's type and memory order;
+    sparse gradients are refused.  One stream at a time may run an optimizer: work that uses it on another stream has to be
+    ordered behind the first, as for any tensor."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, seed=0):
+        if isinstance(lr, torch.Tensor):
+            raise TypeError("lr must be a number")
+        if not lr >= 0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not eps >= 0:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        for i in (0, 1):
+            if not 0 <= betas[i] < 1:
+                raise ValueError(f"Invalid beta parameter at index {i}: {betas[i]}")
+        if not weight_decay >= 0:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, not {state_bits}")
+        self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFFFFFFFFFF
+        self._steps = {}            # group number -> int64 [parameters + 1] on the device: their steps, the kernel's counter
+        self._plans = {}            # group number -> the table of the last step()
+        self._captured = []         # tables (and what they point to) that captured graphs read
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    # ------------------------------------------------------------------------------------------ state
+    def _check_param(self, p):
+        _dtype_code(p, "a parameter")
+        if not _dense(p):
+            raise ValueError("AdamW needs parameters whose elements fill one range of memory")
+        _same_device(p.device)
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        for p in group["params"]:
+            if p.dtype not in _DTYPES:
+                self.param_groups.pop()
+                raise TypeError(f"a parameter must be float32, bfloat16 or float16, not {p.dtype}")
+
+    def _init_state(self, p):
+        self._check_param(p)
+        st = self.state[p]
+        if self.state_bits == 32:
+            for k in ("exp_avg", "exp_avg_sq"):
+                st[k] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            return
+        blocks = -(-p.numel() // _lib.load().sca_adamw_block_elements())
+        for k, f8 in (("exp_avg", _F8_M), ("exp_avg_sq", _F8_V)):
+            st[k] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format).view(f8)
+            st[k + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+
+    def _group_steps(self, gi):
+        ctr = self._steps.get(gi)
+        params = self.param_groups[gi]["params"]
+        if ctr is None:
+            ctr = self._steps[gi] = torch.zeros(len(params) + 1, dtype=torch.int64, device=params[0].device)
+        return ctr
+
+    def set_step(self, step: int):
+        """Set the number of steps that every parameter has behind it (a run taken up from states of another program)."""
+        for gi in range(len(self.param_groups)):
+            self._group_steps(gi)[:-1].fill_(int(step))
+
+    def state_dict(self):
+        """torch's layout; every parameter's state has `step` as a whole number (read from the device)."""
+        sd = super().state_dict()
+        for gi, packed in enumerate(sd["param_groups"]):
+            if gi not in self._steps:
+                continue
+            steps = self._steps[gi].tolist()
+            for i, pid in enumerate(packed["params"]):
+                if pid in sd["state"]:
+                    sd["state"][pid] = dict(sd["state"][pid], step=steps[i])
+        return sd
+
+    def load_state_dict(self, state_dict):
+        """Take up the states of a `state_dict()` of this class with the same state_bits, or (32 bits) of torch.optim.AdamW."""
+        keys = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
+        for st in state_dict["state"].values():
+            if not keys <= set(st) or ("exp_avg_scale" in st) != (self.state_bits == 8):
+                raise ValueError(f"the state dict holds {sorted(st)}, this optimizer keeps {self.state_bits}-bit states")
+        super().load_state_dict(state_dict)
+        self._plans = {}
+        for gi, (group, packed) in enumerate(zip(self.param_groups, state_dict["param_groups"])):
+            steps = []
+            for p, pid in zip(group["params"], packed["params"]):
+                st = state_dict["state"].get(pid)
+                steps.append(int(st.get("step", 0)) if st else 0)
+                if st:      # the types of the states are theirs, not the parameter's
+                    self.state[p] = {k: st[k].to(p.device, torch.float32 if self.state_bits == 32 else st[k].dtype,
+                                                 copy=True) for k in keys}
+            self._group_steps(gi)[:-1].copy_(torch.tensor(steps))
+
+    # ------------------------------------------------------------------------------------------ step
+    def _table(self, gi, group, key):
+        """The device table of a group: entries, chunks, and the tensors that hold them."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step(): the parameters, gradients or states differ from the last call; call it once "
+                               "with them before the capture")
+        lib = _lib.load()
+        chunk = lib.sca_adamw_chunk_elements()
+        block = lib.sca_adamw_block_elements()
+        steps = self._group_steps(gi)
+        first = sum(len(g["params"]) for g in self.param_groups[:gi])
+        dev, rows = steps.device, []
+        for i, p in enumerate(group["params"]):
+            g = p.grad
+            if g is None:
+                continue
+            st = self.state[p]
+            self._check_param(p)
+            if g.is_sparse or g.layout != torch.strided:
+                raise RuntimeError("AdamW does not support sparse gradients")
+            if g.dtype != p.dtype or g.shape != p.shape or _layout(g) != _layout(p):
+                raise ValueError(f"the gradient of parameter {i} is {g.dtype} {tuple(g.shape)} strides {tuple(g.stride())}, "
+                                 f"the parameter {p.dtype} {tuple(p.shape)} strides {tuple(p.stride())}")
+            _same_device(dev, parameter=p, gradient=g, **st)
+            for k, want in (("exp_avg", _F8_M), ("exp_avg_sq", _F8_V)):
+                t = st[k]
+                want = torch.float32 if self.state_bits == 32 else want
+                if t.dtype != want or t.shape != p.shape or _layout(t) != _layout(p):
+                    raise ValueError(f"{k} of parameter {i} must be {want} in the parameter's shape and memory order")
+                if self.state_bits == 8:
+                    s = st[k + "_scale"]
+                    if s.dtype != torch.float32 or s.numel() != -(-p.numel() // block) or not s.is_contiguous():
+                        raise ValueError(f"{k}_scale of parameter {i} must hold one float32 per {block} elements")
+            m, v = st["exp_avg"], st["exp_avg_sq"]
+            size, state_align = p.element_size(), 16 if self.state_bits == 32 else 4
+            vec = not ((p.data_ptr() | g.data_ptr()) % (4 * size) or (m.data_ptr() | v.data_ptr()) % state_align)
+            ms, vs = st.get("exp_avg_scale"), st.get("exp_avg_sq_scale")
+            rows.append(_lib.AdamWTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _lib.ptr(ms), _lib.ptr(vs),
+                                         p.numel(), steps.data_ptr() + 8 * i, float(group["weight_decay"]),
+                                         _DTYPES[p.dtype], int(vec), first + i))
+        counts = np.array([-(-r.n // chunk) for r in rows], dtype=np.int64)
+        chunks = np.empty((int(counts.sum()), 2), dtype=np.int32)
+        chunks[:, 0] = np.repeat(np.arange(len(rows)), counts)
+        chunks[:, 1] = np.arange(len(chunks)) - np.repeat(np.cumsum(counts) - counts, counts)
+        entries = bytes((_lib.AdamWTensor * len(rows))(*rows))
+        # one pinned block, one copy on the current stream (the caching host allocator keeps the block until it has run)
+        host = torch.from_numpy(np.frombuffer(entries + chunks.tobytes(), dtype=np.uint8).copy()).pin_memory()
+        table = host.to(dev, non_blocking=True)
+        at = table.data_ptr()
+        return dict(key=key, table=table, streams={torch.cuda.current_stream(dev).cuda_stream}, entries=at, n=len(rows), chunks=at + len(entries), n_chunks=len(chunks),
+                    steps=steps, done=steps.data_ptr() + 8 * len(group["params"]), device=dev)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        scales = self.state_bits == 8
+        for gi, group in enumerate(self.param_groups):
+            key = [group["weight_decay"]]
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                st = self.state[p]
+                if not st:
+                    self._init_state(p)
+                m, v = st["exp_avg"], st["exp_avg_sq"]
+                key += (p.data_ptr(), p.numel(), p.dtype, g.data_ptr(), g.dtype, _layout(g), m.data_ptr(), v.data_ptr())
+                if scales:
+                    key += (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr())
+            if len(key) == 1:
+                continue
+            plan = self._plans.get(gi)
+            if plan is None or plan["key"] != key:
+                plan = self._plans[gi] = self._table(gi, group, key)
+            if torch.cuda.is_current_stream_capturing():    # replays read the table and what it points to
+                self._captured.append((plan, [(p, p.grad, dict(self.state[p])) for p in group["params"]]))
+            else:
+                stream = torch.cuda.current_stream(plan["device"])
+                if stream.cuda_stream not in plan["streams"]:
+                    plan["streams"].add(stream.cuda_stream)
+                    plan["table"].record_stream(stream)
+            b1, b2 = group["betas"]
+            _call(plan["device"], "sca_adamw_step", plan["entries"], plan["n"], plan["chunks"], plan["n_chunks"],
+                  self.state_bits, None, float(group["lr"]), b1, b2, float(group["eps"]), self.seed, plan["done"])
+        return loss

@@ -1,0 +1,113 @@
+"""What scarches_amd.ops refuses before anything is launched (no GPU needed)."""
+import pytest
+import torch
+
+from scarches_amd import _lib, ops
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("args,error", [
+    ((t(3, 0),), ValueError), ((t(()),), ValueError), ((t(3, 4, dtype=torch.float64),), TypeError),
+    ((t(3, 4, dtype=torch.int32),), TypeError), ((t(3, 4), t(5)), ValueError), ((t(3, 4), t(1, 4)), ValueError),
+    ((t(3, 4), t(4), t(3)), ValueError), ((t(3, 4), None, t(4)), ValueError), ((t(3, 4), t(4, dtype=torch.bfloat16)), TypeError),
+    ((t(3, 4), t(4), t(4, dtype=torch.float16)), TypeError), ((t(3, 4), t(8)[::2]), ValueError), ((t(3, 4), t(4), t(4), -1.0), ValueError),
+    ((t(3, 4), t(4), t(4), float("nan")), ValueError), ((t(3, 4), t(4), t(4)), _lib.HipLibraryError)])
+def test_layer_norm(args, error):
+    with pytest.raises(error):
+        ops.layer_norm_fwd(*args)
+    with pytest.raises(error):
+        ops.layer_norm(*args)
+
+
+@pytest.mark.parametrize("args,error", [
+    ((t(3, 5), t(3, 4), t(4), t(2, 3)), ValueError), ((t(3, 4, dtype=torch.float16), t(3, 4), t(4), t(2, 3)), ValueError),
+    ((t(3, 4), t(3, 4), t(5), t(2, 3)), ValueError), ((t(3, 4), t(3, 4), t(4), t(2, 3)), _lib.HipLibraryError)])
+def test_layer_norm_bwd(args, error):
+    with pytest.raises(error):
+        ops.layer_norm_bwd(*args)
+
+
+I8 = torch.int8
+
+
+@pytest.mark.parametrize("args,error", [
+    ((t(3, 4), t(3), t(5, 4, dtype=I8), t(5)), TypeError), ((t(3, 4, dtype=I8), t(3), t(5, 4), t(5)), TypeError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 6, dtype=I8), t(5)), ValueError), ((t(3, 4, dtype=I8), t(4), t(5, 4, dtype=I8), t(5)), ValueError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 4, dtype=I8), t(4)), ValueError),
+    ((t(3, 4, dtype=I8), t(3, dtype=torch.float16), t(5, 4, dtype=I8), t(5)), ValueError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 4, dtype=I8), t(10)[::2]), ValueError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 4, dtype=I8), t(5), t(4)), ValueError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 4, dtype=I8), t(5), t(5, dtype=torch.float16)), ValueError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 4, dtype=I8), t(5), None, torch.float64), TypeError),
+    ((t(3, 0, dtype=I8), t(3), t(5, 0, dtype=I8), t(5)), ValueError),
+    ((t(1, 1 << 17, dtype=I8), t(1), t(1, 1 << 17, dtype=I8), t(1)), ValueError),
+    ((t(3, 4, dtype=I8), t(3).requires_grad_(), t(5, 4, dtype=I8), t(5)), RuntimeError),
+    ((t(3, 4, dtype=I8), t(3), t(5, 4, dtype=I8), t(5)), _lib.HipLibraryError)])
+def test_int8_matmul(args, error):
+    with pytest.raises(error):
+        ops.int8_matmul(*args)
+
+
+@pytest.mark.parametrize("call,error", [
+    (lambda: ops.int8_linear(t(3, 4).requires_grad_(), t(5, 4, dtype=I8), t(5)), RuntimeError),
+    (lambda: ops.int8_linear(t(3, 4, dtype=torch.float64), t(5, 4, dtype=I8), t(5)), TypeError),
+    (lambda: ops.int8_linear(t(3, 4), t(5, 3, dtype=I8), t(5)), ValueError),
+    (lambda: ops.int8_linear(t(3, 4), t(5, 4, dtype=I8), t(5)), _lib.HipLibraryError),
+    (lambda: ops.quantize_int8(t(3, 0)), ValueError), (lambda: ops.quantize_int8(t(3, 4, dtype=I8)), TypeError),
+    (lambda: ops.quantize_int8(t(3, 4)), _lib.HipLibraryError)])
+def test_int8_linear(call, error):
+    with pytest.raises(error):
+        call()
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(lr=-1.0), ValueError), (dict(lr=torch.tensor(1.0)), TypeError), (dict(eps=-1e-8), ValueError), (dict(betas=(1.0, 0.9)), ValueError),
+    (dict(betas=(0.9, -0.1)), ValueError), (dict(weight_decay=-0.1), ValueError), (dict(state_bits=16), ValueError)])
+def test_adamw_arguments(kw, error):
+    with pytest.raises(error):
+        ops.AdamW([t(3)], **kw)
+
+
+def test_adamw_parameters():
+    with pytest.raises(TypeError):
+        ops.AdamW([t(3, dtype=torch.float64)])
+    with pytest.raises(ValueError):                 # the same tensor twice in a group, or in two
+        p = t(3)
+        ops.AdamW([dict(params=[p]), dict(params=[p])])
+    p = t(3)
+    opt = ops.AdamW([p])
+    opt.step()                                      # nothing has a gradient: nothing to do
+    p.grad = t(3)
+    with pytest.raises(_lib.HipLibraryError):
+        opt.step()
+    q = t(3, 4).expand(2, 3, 4)
+    q.grad = t(2, 3, 4)
+    with pytest.raises(ValueError, match="one range of memory"):
+        ops.AdamW([q]).step()
+
+
+def test_entry_points_check_their_arguments():
+    """-1 from the C entry points, before a kernel is launched (the addresses are never read)."""
+    lib = _lib.load()
+    a = 4096
+    ok = (a, 8, 0, 4, 8, a, a, 0, 1e-5, a, 8, a, None)
+    for i, bad in ((0, None), (1, -1), (2, 3), (3, -1), (4, 0), (7, 1), (8, -1.0), (9, None), (10, 7)):
+        assert lib.sca_layernorm_fwd(*ok[:i], bad, *ok[i + 1:]) == -1, i
+    ok = (a, 8, a, 8, 0, 4, 8, a, 0, a, a, 8, a, a, a, None)
+    for i, bad in ((0, None), (1, -1), (2, None), (3, -1), (4, 7), (5, -1), (6, 0), (8, 2), (9, None), (11, 7), (14, None)):
+        assert lib.sca_layernorm_bwd(*ok[:i], bad, *ok[i + 1:]) == -1, i
+    assert lib.sca_layernorm_bwd_workspace_floats(-1, 3) == -1 and lib.sca_layernorm_bwd_workspace_floats(5, 0) == -1
+    ok = (a, 8, 0, 4, 8, a, 8, a, None)
+    for i, bad in ((0, None), (1, -1), (2, 5), (3, -1), (4, 0), (5, None), (6, 7), (7, None)):
+        assert lib.sca_quant_rows_i8(*ok[:i], bad, *ok[i + 1:]) == -1, i
+    ok = (a, 8, a, a, 8, a, a, 0, 4, 5, 8, a, 0, 5, None)
+    for i, bad in ((0, None), (1, -1), (2, None), (3, None), (4, 7), (5, None), (7, 1), (8, -1), (9, -1), (10, 0),
+                   (10, lib.sca_gemm_i8_max_k() + 1), (11, None), (12, 3), (13, 4)):
+        assert lib.sca_gemm_i8(*ok[:i], bad, *ok[i + 1:]) == -1, i
+    ok = (a, 1, a, 1, 32, None, 1e-3, 0.9, 0.999, 1e-8, 0, a, None)
+    for i, bad in ((0, None), (1, -1), (2, None), (3, -1), (4, 16), (7, 1.0), (8, -0.1), (9, -1.0), (11, None)):
+        assert lib.sca_adamw_step(*ok[:i], bad, *ok[i + 1:]) == -1, i
+    assert lib.sca_adamw_step(a, 1, a, 1, 8, a, 1e-3, 0.9, 0.999, 1e-8, 0, None, None) == -1      # hyper: 32 bits only
