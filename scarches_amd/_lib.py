@@ -154,6 +154,8 @@ SIGNATURES = {
     "sca_gemm_i8_max_k": [],
     "sca_quant_rows_i8": [P, LL, I, LL, I, P, LL, P, P],
     "sca_gemm_i8": [P, LL, P, P, LL, P, P, I, LL, I, I, P, I, LL, P],
+    "sca_linear_i8_workspace_bytes": [LL, I],
+    "sca_linear_i8": [P, LL, I, P, LL, P, P, I, LL, I, I, P, I, LL, P, P],
     "sca_embed_lookup": [P, I, I, P, I, I, F, P, P, I, P],
     "sca_embed_scatter_add": [P, P, I, I, I, I, P, I, P, P],
     "sca_proto_workspace_bytes": [I, I, I],
@@ -163,7 +165,7 @@ SIGNATURES = {
     "sca_class_moments_finish": [P, P, P, I, I, P, P, P, P, P, P],
 }
 RESTYPES = {"sca_hsic_workspace_floats": LL, "sca_proto_workspace_bytes": LL, "sca_knn_static_max_entries": LL,
-            "sca_layernorm_bwd_workspace_floats": LL}
+            "sca_layernorm_bwd_workspace_floats": LL, "sca_linear_i8_workspace_bytes": LL}
 
 _lib = None
 ABI_VERSION = 3       # sca_abi_version() of the library this binding was written against

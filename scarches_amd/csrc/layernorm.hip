@@ -5,121 +5,418 @@
 //
 // fp32 / bf16 / fp16 rows of any width and pitch; statistics, sums and gradients are held in fp32 and rounded once when
 // they are stored.  (sca_layer_fwd / sca_layer_bwd normalise without weight and bias inside the conditional layers.)
+//
+// All passes are bound by memory, so a row is read once: TPR threads (16 ... 1024, as wide as the row needs) hold it in
+// registers, the mean and then the squared distances from it are summed from there.  The backward pass keeps the column
+// sums of dw and db in registers over all rows that a thread walks and leaves one slab of partial sums per workgroup, so
+// that they cost no second pass over x and dy; a second launch adds the slabs in a fixed order (no atomics).
 #include "common.h"
 #include "dtypes.h"
+#include "rowtile.h"
 
 namespace {
 
-// One wave per row, three passes over the row.
+constexpr long long MAX_BLOCKS = 1 << 20;        // a launch holds fewer than 2^32 threads; rows beyond it are looped over
+
+// Weight elements [c, c + VEC) of n (type W, so up to 32 bytes), `other` where there is no weight.
+template <int MODE, typename W, int VEC>
+__device__ __forceinline__ void load_weight(const W* __restrict__ w, int c, int n, float other, float (&v)[VEC]) {
+    if (w) {
+        if (MODE == ROW_TINY) load_part<W, VEC>(w, n, v);
+        else load_vec<W, VEC>(w + c, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = other;
+    }
+}
+
+template <typename T, typename W, int TPR, int V, int MODE>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_kernel(const T* __restrict__ x, long long ldx,
+                                                                       long long rows, int n, const W* __restrict__ w,
+                                                                       const W* __restrict__ b, float eps,
+                                                                       T* __restrict__ y, long long ldy,
+                                                                       float* __restrict__ stats) {
+    constexpr int VEC = vec_of<T>(), NT = TPR > 256 ? TPR : 256;
+    __shared__ float scratch[16];
+    const int t = threadIdx.x % TPR;
+    for (long long r = (long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR; r < rows;
+         r += (long long)gridDim.x * (NT / TPR)) {
+        const T* xr = x + r * ldx;
+        raw_t raw[V] = {};
+        float v[VEC];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (at.there) load_cols<MODE>(xr, at.c, n, raw[j]);
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            unpack<T>(raw[j], v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s += at.own(i, n) ? v[i] : 0.f;        // (a vector that is not there is 0)
+        }
+        const float mean = row_sum<TPR>(s, scratch) / (float)n;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            unpack_again<T>(raw[j], v);
+            float p = 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float d = at.own(i, n) ? v[i] - mean : 0.f;
+                p = fmaf(d, d, p);
+            }
+            q += at.there ? p : 0.f;
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, scratch) / (float)n + eps);
+        T* yr = y + r * ldy;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (!at.there) continue;
+            float g[VEC], o[VEC];
+            load_weight<MODE>(w, at.c, n, 1.f, g);
+            load_weight<MODE>(b, at.c, n, 0.f, o);
+            unpack_again<T>(raw[j], v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, g[i], o[i]);
+            store_cols<MODE>(yr, at.c, n, v);
+        }
+        if (t == 0 && stats) {
+            stats[r] = mean;
+            stats[rows + r] = rstd;
+        }
+    }
+}
+
+// Rows beyond what a workgroup's registers hold: one workgroup per row, three passes (the later ones from a cache).
 template <typename T, typename W>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, long long ldx, long long rows, int n,
-                                                     const W* __restrict__ w, const W* __restrict__ b, float eps,
-                                                     T* __restrict__ y, long long ldy, float* __restrict__ stats) {
-    const int lane = threadIdx.x & 63;
-    const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, long long ldx, long long rows, int n,
+                                                           const W* __restrict__ w, const W* __restrict__ b, float eps,
+                                                           T* __restrict__ y, long long ldy, float* __restrict__ stats) {
+    constexpr int VEC = vec_of<T>();
+    __shared__ float scratch[16];
+    const long long r = blockIdx.x;              // (rows this long are fewer than a grid holds)
     const T* xr = x + r * ldx;
-    float s = 0.f;
-    for (int c = lane; c < n; c += 64) s += to_f32(xr[c]);
-    const float mean = wave_sum(s) / (float)n;
-    float q = 0.f;
-    for (int c = lane; c < n; c += 64) {
-        const float d = to_f32(xr[c]) - mean;
-        q = fmaf(d, d, q);
+    const int vecs = (n + VEC - 1) / VEC;
+    float v[VEC], s = 0.f, q = 0.f;
+    auto col = [&](int j) { return j * VEC < n - VEC ? j * VEC : n - VEC; };
+    for (int j = threadIdx.x; j < vecs; j += 1024) {
+        const int skip = j * VEC - col(j);
+        load_vec<T, VEC>(xr + col(j), v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s += i >= skip ? v[i] : 0.f;
     }
-    const float rstd = 1.0f / sqrtf(wave_sum(q) / (float)n + eps);
-    for (int c = lane; c < n; c += 64) {
-        float v = (to_f32(xr[c]) - mean) * rstd;
-        if (w) v *= to_f32(w[c]);
-        if (b) v += to_f32(b[c]);
-        y[r * ldy + c] = from_f32<T>(v);
+    const float mean = row_sum<1024>(s, scratch) / (float)n;
+    for (int j = threadIdx.x; j < vecs; j += 1024) {
+        const int skip = j * VEC - col(j);
+        load_vec<T, VEC>(xr + col(j), v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float d = i >= skip ? v[i] - mean : 0.f;
+            q = fmaf(d, d, q);
+        }
     }
-    if (lane == 0 && stats) {
+    const float rstd = 1.0f / sqrtf(row_sum<1024>(q, scratch) / (float)n + eps);
+    for (int j = threadIdx.x; j < vecs; j += 1024) {
+        float g[VEC], o[VEC];
+        load_weight<ROW_RAGGED>(w, col(j), n, 1.f, g);
+        load_weight<ROW_RAGGED>(b, col(j), n, 0.f, o);
+        load_vec<T, VEC>(xr + col(j), v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, g[i], o[i]);
+        store_vec<T, VEC>(y + r * ldy + col(j), v);
+    }
+    if (threadIdx.x == 0 && stats) {
         stats[r] = mean;
         stats[rows + r] = rstd;
     }
 }
 
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void ln_dx_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ x,
-                                                    long long ldx, long long rows, int n, const W* __restrict__ w,
-                                                    const float* __restrict__ stats, T* __restrict__ dx, long long lddx) {
-    const int lane = threadIdx.x & 63;
-    const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
-    const float mean = stats[r], rstd = stats[rows + r];
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = lane; c < n; c += 64) {
-        const float a = to_f32(dy[r * lddy + c]) * (w ? to_f32(w[c]) : 1.f);
-        s1 += a;
-        s2 = fmaf(a, (to_f32(x[r * ldx + c]) - mean) * rstd, s2);
+// ---- backward ---------------------------------------------------------------------------------------------------------
+struct LnBwd {
+    const void* dy; long long lddy;
+    const void* x; long long ldx;
+    long long rows; int n;
+    const void* w;
+    const float* stats;
+    void* dx; long long lddx;
+    float* part;                 // [slab][2][n] partial sums of (dw, db), or null
+};
+
+// Threads of a workgroup: eight waves of rows of up to 64 threads each, or one row.
+template <int TPR>
+constexpr int bwd_threads() { return TPR > 64 ? TPR : 512; }
+
+template <typename T, typename W, int TPR, int V, int MODE>
+__global__ __launch_bounds__(bwd_threads<TPR>()) void ln_bwd_kernel(const LnBwd a) {
+    constexpr int VEC = vec_of<T>(), NT = bwd_threads<TPR>(), PER = NT / TPR;
+    __shared__ float scratch[16];
+    __shared__ float sums[TPR > 64 ? 1 : 2 * TPR * V * VEC];     // (one row per workgroup: nothing to add up)
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, n = a.n;
+    const float inv_n = 1.f / (float)n;
+    float g[V][VEC], dw[V][VEC], db[V][VEC];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const Cols<T, TPR, MODE> at(j, t, n);
+        if (at.there) load_weight<MODE>((const W*)a.w, at.c, n, 1.f, g[j]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) dw[j][i] = db[j][i] = 0.f;
     }
-    const float m1 = wave_sum(s1) / (float)n, m2 = wave_sum(s2) / (float)n;
-    for (int c = lane; c < n; c += 64) {
-        const float a = to_f32(dy[r * lddy + c]) * (w ? to_f32(w[c]) : 1.f);
-        const float h = (to_f32(x[r * ldx + c]) - mean) * rstd;
-        dx[r * lddx + c] = from_f32<T>(rstd * (a - m1 - h * m2));
+    for (long long r = (long long)blockIdx.x * PER + sub; r < a.rows; r += (long long)gridDim.x * PER) {
+        const T *xr = (const T*)a.x + r * a.ldx, *dr = (const T*)a.dy + r * a.lddy;
+        raw_t xq[V] = {}, dq[V] = {};
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (at.there) {
+                load_cols<MODE>(xr, at.c, n, xq[j]);
+                load_cols<MODE>(dr, at.c, n, dq[j]);
+            }
+        }
+        const float mean = a.stats[r], rstd = a.stats[a.rows + r];
+        float s1 = 0.f, s2 = 0.f, h[VEC], d[VEC];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (!at.there) continue;
+            unpack<T>(xq[j], h);
+            unpack<T>(dq[j], d);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                h[i] = (h[i] - mean) * rstd;
+                dw[j][i] = fmaf(d[i], h[i], dw[j][i]);
+                db[j][i] += d[i];
+                const float p = at.own(i, n) ? d[i] * g[j][i] : 0.f;
+                s1 += p;
+                s2 = fmaf(p, h[i], s2);
+            }
+        }
+        if (!a.dx) continue;
+        const float m1 = row_sum<TPR>(s1, scratch) * inv_n, m2 = row_sum<TPR>(s2, scratch) * inv_n;
+        T* out = (T*)a.dx + r * a.lddx;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (!at.there) continue;
+            unpack_again<T>(xq[j], h);
+            unpack_again<T>(dq[j], d);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) d[i] = rstd * (fmaf(d[i], g[j][i], -m1) - (h[i] - mean) * rstd * m2);
+            store_cols<MODE>(out, at.c, n, d);
+        }
+    }
+    if (!a.part) return;
+    float* slab = a.part + (long long)blockIdx.x * 2 * n;
+    if constexpr (TPR > 64) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (!at.there) continue;
+            store_vec<float, VEC>(slab + at.c, dw[j]);
+            store_vec<float, VEC>(slab + n + at.c, db[j]);
+        }
+    } else {
+        // the workgroup's rows one after the other into LDS (vectors, columns as the threads hold them)
+        for (int k = 0; k < PER; ++k) {
+            __syncthreads();
+            if (sub != k) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int o = (j * VEC + i) * TPR + t;
+                    sums[o] = k ? sums[o] + dw[j][i] : dw[j][i];
+                    sums[TPR * V * VEC + o] = k ? sums[TPR * V * VEC + o] + db[j][i] : db[j][i];
+                }
+        }
+        __syncthreads();
+        if (sub) return;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Cols<T, TPR, MODE> at(j, t, n);
+            if (!at.there) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int o = (j * VEC + i) * TPR + t;
+                dw[j][i] = sums[o];
+                db[j][i] = sums[TPR * V * VEC + o];
+            }
+            if (MODE == ROW_TINY) {
+                store_part<float, VEC>(slab, n, dw[j]);
+                store_part<float, VEC>(slab + n, n, db[j]);
+            } else {
+                store_vec<float, VEC>(slab + at.c, dw[j]);
+                store_vec<float, VEC>(slab + n + at.c, db[j]);
+            }
+        }
     }
 }
 
-constexpr int LN_SLABS = 256;       // row ranges of the weight gradients, summed in a fixed order
-
+// Rows beyond the registers: one workgroup per row for dx, and columns by slabs of rows for dw and db.
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void ln_dx_long_kernel(const LnBwd a) {
+    constexpr int VEC = vec_of<T>();
+    __shared__ float scratch[16];
+    const long long r = blockIdx.x;
+    const int n = a.n, vecs = (n + VEC - 1) / VEC;
+    const T *xr = (const T*)a.x + r * a.ldx, *dr = (const T*)a.dy + r * a.lddy;
+    const float mean = a.stats[r], rstd = a.stats[a.rows + r], inv_n = 1.f / (float)n;
+    float h[VEC], d[VEC], g[VEC], s1 = 0.f, s2 = 0.f;
+    auto col = [&](int j) { return j * VEC < n - VEC ? j * VEC : n - VEC; };
+    for (int j = threadIdx.x; j < vecs; j += 1024) {
+        const int skip = j * VEC - col(j);
+        load_vec<T, VEC>(xr + col(j), h);
+        load_vec<T, VEC>(dr + col(j), d);
+        load_weight<ROW_RAGGED>((const W*)a.w, col(j), n, 1.f, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float p = i >= skip ? d[i] * g[i] : 0.f;
+            s1 += p;
+            s2 = fmaf(p, (h[i] - mean) * rstd, s2);
+        }
+    }
+    const float m1 = row_sum<1024>(s1, scratch) * inv_n, m2 = row_sum<1024>(s2, scratch) * inv_n;
+    for (int j = threadIdx.x; j < vecs; j += 1024) {
+        load_vec<T, VEC>(xr + col(j), h);
+        load_vec<T, VEC>(dr + col(j), d);
+        load_weight<ROW_RAGGED>((const W*)a.w, col(j), n, 1.f, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d[i] = rstd * (fmaf(d[i], g[i], -m1) - (h[i] - mean) * rstd * m2);
+        store_vec<T, VEC>((T*)a.dx + r * a.lddx + col(j), d);
+    }
+}
 template <typename T>
-__global__ __launch_bounds__(256) void ln_dw_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ x,
-                                                    long long ldx, long long rows, int n,
-                                                    const float* __restrict__ stats, float* __restrict__ part) {
+__global__ __launch_bounds__(256) void ln_dw_long_kernel(const LnBwd a) {
     const int c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= n) return;
-    const long long per = (rows + gridDim.x - 1) / gridDim.x;
-    const long long r0 = blockIdx.x * per, r1 = r0 + per < rows ? r0 + per : rows;
+    if (c >= a.n) return;
+    const long long per = (a.rows + gridDim.x - 1) / gridDim.x;
+    const long long r0 = blockIdx.x * per, r1 = r0 + per < a.rows ? r0 + per : a.rows;
     float sw = 0.f, sb = 0.f;
     for (long long r = r0; r < r1; ++r) {
-        const float d = to_f32(dy[r * lddy + c]);
-        sw = fmaf(d, (to_f32(x[r * ldx + c]) - stats[r]) * stats[rows + r], sw);
+        const float d = to_f32(((const T*)a.dy)[r * a.lddy + c]);
+        sw = fmaf(d, (to_f32(((const T*)a.x)[r * a.ldx + c]) - a.stats[r]) * a.stats[a.rows + r], sw);
         sb += d;
     }
-    part[(long long)blockIdx.x * 2 * n + c] = sw;
-    part[(long long)blockIdx.x * 2 * n + n + c] = sb;
+    a.part[(long long)blockIdx.x * 2 * a.n + c] = sw;
+    a.part[(long long)blockIdx.x * 2 * a.n + a.n + c] = sb;
 }
 
+// dw and db from the slabs: 64 columns per workgroup, 16 threads a column, added in a fixed order.
 template <typename W>
-__global__ __launch_bounds__(256) void ln_dw_finish_kernel(const float* __restrict__ part, int slabs, int n,
-                                                           W* __restrict__ dw, W* __restrict__ db) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
-    float sw = 0.f, sb = 0.f;
-    for (int s = 0; s < slabs; ++s) {
-        sw += part[(long long)s * 2 * n + c];
-        sb += part[(long long)s * 2 * n + n + c];
-    }
-    if (dw) dw[c] = from_f32<W>(sw);
-    if (db) db[c] = from_f32<W>(sb);
+__global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restrict__ part, int slabs, int n,
+                                                            W* __restrict__ dw, W* __restrict__ db) {
+    __shared__ float sum[16][64];
+    const int lane = threadIdx.x & 63, k = threadIdx.x >> 6;
+    const long long c = (long long)blockIdx.x * 64 + lane;       // column of [dw | db]
+    float v = 0.f;
+    if (c < 2LL * n)
+        for (int s = k; s < slabs; s += 16) v += part[(long long)s * 2 * n + c];
+    sum[k][lane] = v;
+    __syncthreads();
+    if (k || c >= 2LL * n) return;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v += sum[i][lane];
+    W* out = c < n ? dw : db;
+    if (out) out[c < n ? c : c - n] = from_f32<W>(v);
 }
 
-int ln_slabs(long long rows) { return rows < LN_SLABS ? (int)(rows > 0 ? rows : 1) : LN_SLABS; }
+// ---- launches ---------------------------------------------------------------------------------------------------------
+constexpr int CUS = 256;
+
+// How a row of `vecs` vectors is held: TPR threads, V vectors each (the backward pass keeps five values per element).
+// Slabs of partial sums of the weight gradients: one workgroup per CU walks the rows, as many workgroups as there are rows
+// to fill them.
+struct BwdShape { int tpr, slabs; };
+BwdShape bwd_shape(long long rows, int n, int vec) {
+    const int vecs = (n + vec - 1) / vec, v = 32 / vec;
+    BwdShape s;
+    s.tpr = vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 * v ? 64 : vecs <= 256 * v ? 256 : n <= 16384 ? 1024 : 0;
+    const int per = s.tpr == 0 ? 1 : s.tpr > 64 ? 1 : 512 / s.tpr;
+    const long long blocks = (rows + per - 1) / per;
+    const int most = s.tpr == 256 ? 2 * CUS : CUS;
+    s.slabs = (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+    return s;
+}
 
 template <typename T, typename W>
 int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, const void* b, float eps, void* y,
            long long ldy, float* stats, hipStream_t st) {
-    hipLaunchKernelGGL((ln_fwd_kernel<T, W>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, (const T*)x, ldx, rows,
-                       n, (const W*)w, (const W*)b, eps, (T*)y, ldy, stats);
+    constexpr int VEC = vec_of<T>();
+    const int vecs = (n + VEC - 1) / VEC, mode = row_mode(n, VEC);
+#define FWD_MODE(TPR, V, MODE)                                                                                           \
+    hipLaunchKernelGGL((ln_fwd_kernel<T, W, TPR, V, MODE>), dim3((unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS)), \
+                       dim3(NT), 0, st, (const T*)x, ldx, rows, n, (const W*)w, (const W*)b, eps, (T*)y, ldy, stats)
+#define FWD(TPR, V)                                                             \
+    do {                                                                        \
+        constexpr int NT = TPR > 256 ? TPR : 256;                               \
+        const long long blocks = (rows + NT / TPR - 1) / (NT / TPR);            \
+        if (mode == ROW_FULL) FWD_MODE(TPR, V, ROW_FULL);                       \
+        else FWD_MODE(TPR, V, ROW_RAGGED);                                      \
+    } while (0)
+    if (mode == ROW_TINY) {
+        constexpr int NT = 256;
+        const long long blocks = (rows + 15) / 16;
+        FWD_MODE(16, 1, ROW_TINY);
+    }
+    // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory.
+    else if (vecs <= 16) FWD(16, 1);
+    else if (vecs <= 32) FWD(32, 1);
+    else if (vecs <= 64) FWD(64, 1);
+    else if (vecs <= 128) FWD(64, 2);
+    else if (vecs <= 256 && rows < 4096) FWD(256, 1);
+    else if (vecs <= 256) FWD(64, 4);
+    else if (vecs <= 512 && rows < 4096) FWD(256, 2);
+    else if (vecs <= 512) FWD(64, 8);
+    else if (vecs <= 1024 && rows < 1024) FWD(1024, 1);
+    else if (vecs <= 1024) FWD(256, 4);
+    else if (vecs <= 2048) FWD(1024, 2);
+    else if (vecs <= 4096) FWD(1024, 4);
+    else
+        hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)rows), dim3(1024), 0, st, (const T*)x, ldx, rows, n,
+                           (const W*)w, (const W*)b, eps, (T*)y, ldy, stats);
+#undef FWD
+#undef FWD_MODE
     SCA_CHECK_LAUNCH();
     return 0;
 }
 
 template <typename T, typename W>
-int ln_bwd(const void* dy, long long lddy, const void* x, long long ldx, long long rows, int n, const void* w,
-           const float* stats, void* dx, long long lddx, void* dw, void* db, float* ws, hipStream_t st) {
-    if (rows > 0 && dx)
-        hipLaunchKernelGGL((ln_dx_kernel<T, W>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, (const T*)dy, lddy,
-                           (const T*)x, ldx, rows, n, (const W*)w, stats, (T*)dx, lddx);
-    if (dw || db) {
-        const int slabs = ln_slabs(rows);
-        hipLaunchKernelGGL((ln_dw_kernel<T>), dim3(slabs, (n + 255) / 256), dim3(256), 0, st, (const T*)dy, lddy,
-                           (const T*)x, ldx, rows, n, stats, ws);
-        hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((n + 255) / 256), dim3(256), 0, st, ws, slabs, n, (W*)dw,
-                           (W*)db);
+int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
+    constexpr int VEC = vec_of<T>(), V = 32 / VEC;
+    const int n = a.n, vecs = (n + VEC - 1) / VEC, mode = row_mode(n, VEC);
+    const BwdShape sh = bwd_shape(a.rows, n, VEC);
+    if (a.rows > 0 && sh.tpr) {
+#define BWD_MODE(TPR, V, MODE)                                                                                            \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, W, TPR, V, MODE>), dim3((unsigned)grid), dim3(bwd_threads<TPR>()), 0, st, a)
+#define BWD(TPR, V)                                         \
+    do {                                                    \
+        if (mode == ROW_FULL) BWD_MODE(TPR, V, ROW_FULL);   \
+        else BWD_MODE(TPR, V, ROW_RAGGED);                  \
+    } while (0)
+        const int grid = sh.slabs;
+        if (mode == ROW_TINY) BWD_MODE(16, 1, ROW_TINY);
+        else if (vecs <= 16) BWD(16, 1);
+        else if (vecs <= 32) BWD(32, 1);
+        else if (vecs <= 64) BWD(64, 1);
+        else if (V > 4 && vecs <= 64 * 4) BWD(64, (V > 4 ? 4 : V));
+        else if (vecs <= 64 * V) BWD(64, V);
+        else if (vecs <= 256 * V) BWD(256, V);
+        else BWD(1024, V / 2);
+#undef BWD
+#undef BWD_MODE
+    } else if (a.rows > 0) {
+        if (a.dx) hipLaunchKernelGGL((ln_dx_long_kernel<T, W>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+        if (a.part)
+            hipLaunchKernelGGL((ln_dw_long_kernel<T>), dim3(sh.slabs, (n + 255) / 256), dim3(256), 0, st, a);
     }
+    if (dw || db)
+        hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((unsigned)((2LL * n + 63) / 64)), dim3(1024), 0, st, a.part,
+                           a.rows > 0 ? sh.slabs : 0, n, (W*)dw, (W*)db);
     SCA_CHECK_LAUNCH();
     return 0;
 }
@@ -147,7 +444,9 @@ extern "C" int sca_layernorm_fwd(const void* x, long long ldx, int dtype, long l
 }
 
 extern "C" long long sca_layernorm_bwd_workspace_floats(long long rows, int n) {
-    return rows < 0 || n <= 0 ? -1 : 2LL * n * ln_slabs(rows);
+    if (rows < 0 || n <= 0) return -1;
+    const int a = bwd_shape(rows, n, 4).slabs, b = bwd_shape(rows, n, 8).slabs;      // whatever the type
+    return 2LL * n * (a > b ? a : b);
 }
 
 extern "C" int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, int dtype,
@@ -156,5 +455,7 @@ extern "C" int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, 
     if (!ln_types_ok(dtype, wtype) || rows < 0 || n <= 0 || lddy < 0 || ldx < 0 || (dx && lddx < n)) return -1;
     if (rows > 0 && (!dy || !x || !stats)) return -1;
     if ((dw || db) && !ws) return -1;
-    return LN_DISPATCH(ln_bwd, dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, dw, db, ws, (hipStream_t)stream);
+    if (!dx && !dw && !db) return 0;
+    const LnBwd a{dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, dw || db ? ws : nullptr};
+    return LN_DISPATCH(ln_bwd, a, dw, db, (hipStream_t)stream);
 }

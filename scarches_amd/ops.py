@@ -201,16 +201,12 @@ def _no_grad(*tensors):
         raise RuntimeError("the 8-bit integer product is for serving and has no gradient: call it under torch.no_grad()")
 
 
-def _i8_product(xq_ptr, ldx, sx_ptr, wq, w_scale, bias, shape, rows, k, out_dtype):
-    n = wq.shape[0]
-    y = torch.empty((*shape, n), dtype=out_dtype, device=wq.device)
-    if rows and n:
-        if k > 1 and wq.stride(1) != 1:
-            wq = wq.contiguous()
-        _call(wq.device, "sca_gemm_i8", xq_ptr, ldx, sx_ptr, wq.data_ptr(), wq.stride(0) if n > 1 else k, w_scale.data_ptr(),
-              _lib.ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], rows, n, k, y.data_ptr(),
-              _DTYPES[out_dtype], n)
-    return y
+def _weight_rows(wq):
+    """(wq with contiguous rows, their pitch)."""
+    n, k = wq.shape
+    if k > 1 and wq.stride(1) != 1:
+        wq = wq.contiguous()
+    return wq, wq.stride(0) if n > 1 else k
 
 
 def int8_matmul(xq, x_scale, wq, w_scale, bias: Optional[torch.Tensor] = None, out_dtype=torch.float32):
@@ -226,7 +222,13 @@ def int8_matmul(xq, x_scale, wq, w_scale, bias: Optional[torch.Tensor] = None, o
     _no_grad(x_scale, w_scale, bias)
     _same_device(wq.device, xq=xq, x_scale=x_scale, w_scale=w_scale, bias=bias)
     x2, rows, ldx = _rows(xq)
-    return _i8_product(x2.data_ptr(), ldx, x_scale.data_ptr(), wq, w_scale, bias, xq.shape[:-1], rows, k, out_dtype)
+    wq, ldw = _weight_rows(wq)
+    n = wq.shape[0]
+    y = torch.empty((*xq.shape[:-1], n), dtype=out_dtype, device=wq.device)
+    if rows and n:
+        _call(wq.device, "sca_gemm_i8", x2.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw, w_scale.data_ptr(),
+              _lib.ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], rows, n, k, y.data_ptr(), _DTYPES[out_dtype], n)
+    return y
 
 
 def int8_linear(x, wq, w_scale, bias: Optional[torch.Tensor] = None, out_dtype=None):
@@ -242,12 +244,15 @@ def int8_linear(x, wq, w_scale, bias: Optional[torch.Tensor] = None, out_dtype=N
     dev = x.device
     _same_device(dev, wq=wq, w_scale=w_scale, bias=bias)
     x2, rows, ldx = _rows(x)
-    pitch = -(-k // _PAD_K) * _PAD_K
-    buf = torch.empty(rows * (pitch + 4), dtype=torch.int8, device=dev)    # the quantized rows, then their scales
-    q_ptr, scale_ptr = buf.data_ptr(), buf.data_ptr() + rows * pitch
-    if rows:
-        _call(dev, "sca_quant_rows_i8", x2.data_ptr(), ldx, code, rows, k, q_ptr, pitch, scale_ptr)
-    return _i8_product(q_ptr, pitch, scale_ptr, wq, w_scale, bias, x.shape[:-1], rows, k, out_dtype)
+    wq, ldw = _weight_rows(wq)
+    n = wq.shape[0]
+    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=dev)
+    if rows and n:
+        size = _lib.load().sca_linear_i8_workspace_bytes(rows, k)
+        ws = torch.empty(size, dtype=torch.int8, device=dev) if size else None
+        _call(dev, "sca_linear_i8", x2.data_ptr(), ldx, code, wq.data_ptr(), ldw, w_scale.data_ptr(), _lib.ptr(bias),
+              0 if bias is None else _DTYPES[bias.dtype], rows, n, k, y.data_ptr(), _DTYPES[out_dtype], n, _lib.ptr(ws))
+    return y
 
 
 # ---------------------------------------------------------------------------------------------- AdamW

@@ -406,6 +406,27 @@ def test_int8_offsets_past_32_bits(ops):
     assert torch.equal(q[-1:], tq) and torch.equal(s[-1:], ts) and not s[:-1].any()
 
 
+def test_more_rows_than_a_grid_holds(ops):
+    """70 million short rows: 2^32 threads are not enough to give each its own."""
+    rows = 70_000_000
+    x = torch.arange(rows, device="cuda", dtype=torch.float32)[:, None] * torch.tensor([1.0, -0.5, 0.25], device="cuda")
+    q, s = ops.quantize_int8(x)
+    # (-0.5 and 0.25 of the largest value are -63.5 and 31.75 scales up to the scale's rounding: which integer -63.5 goes to
+    # depends on it, so the reference is the quotient in 64 bits)
+    same = bool((s == x[:, 0] / torch.full_like(s, 127)).all())
+    ref = torch.round(x[1:].double() / s[1:, None].double())
+    same = same and bool((q[1:] == ref).all()) and not bool(q[0].any())
+    assert same
+    del q, s, ref
+    y, stats = ops.layer_norm_fwd(x)
+    at = torch.tensor([0, 1, 5, 67_108_863, 67_108_864, rows - 1], device="cuda")
+    want, _ = ops.layer_norm_fwd(x[at])
+    assert torch.equal(y[at], want) and torch.equal(stats[0, at], ops.layer_norm_fwd(x[at])[1][0])
+    assert (y[2:, 0] > 1).all()
+    dx, _, _ = ops.layer_norm_bwd(y, x, None, stats)
+    assert torch.equal(dx[at], ops.layer_norm_bwd(want, x[at], None, stats[:, at].contiguous())[0])
+
+
 # ---------------------------------------------------------------------------------------------- AdamW
 LR, B1, B2, EPS, WD = 3e-3, 0.9, 0.999, 1e-8, 0.05
 
