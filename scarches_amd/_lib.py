@@ -150,6 +150,7 @@ SIGNATURES = {
     "sca_layernorm_bwd": [P, LL, P, LL, I, LL, I, P, I, P, P, LL, P, P, P, P],
     "sca_adamw_chunk_elements": [],
     "sca_adamw_block_elements": [],
+    "sca_adamw_scratch_bytes": [I],
     "sca_adamw_step": [P, I, P, I, I, P, F, D, D, F, U64, P, P],
     "sca_gemm_i8_max_k": [],
     "sca_quant_rows_i8": [P, LL, I, LL, I, P, LL, P, P],
@@ -165,7 +166,8 @@ SIGNATURES = {
     "sca_class_moments_finish": [P, P, P, I, I, P, P, P, P, P, P],
 }
 RESTYPES = {"sca_hsic_workspace_floats": LL, "sca_proto_workspace_bytes": LL, "sca_knn_static_max_entries": LL,
-            "sca_layernorm_bwd_workspace_floats": LL, "sca_linear_i8_workspace_bytes": LL}
+            "sca_layernorm_bwd_workspace_floats": LL, "sca_linear_i8_workspace_bytes": LL,
+            "sca_adamw_scratch_bytes": LL}
 
 _lib = None
 ABI_VERSION = 3       # sca_abi_version() of the library this binding was written against

@@ -3,9 +3,10 @@
 //   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)        (decoupled decay)
 //
-// A launch walks a table of tensors that lies in device memory (one entry per tensor, one per chunk of 2048 elements), so
-// the number of tensors costs no launches.  The step number lives in device memory as well: the last workgroup to finish
-// advances it, so a captured step counts on when it is replayed.
+// A step walks a table of tensors that lies in device memory (one entry per tensor, one per chunk of 2048 elements), so
+// the number of tensors costs no launches.  The step numbers live in device memory as well: a small launch in front
+// advances them and derives every tensor's coefficients (in 64 bits, once, instead of in every workgroup), so a captured
+// step counts on when it is replayed.
 //
 // 8-bit states: every 256 elements of a tensor share a power-of-two scale per moment, with m / scale held as e4m3 and
 // v / scale as e5m2 floats (v spans twice the exponents of m).  Rounding to that grid is stochastic: at b2 = 0.999 a step
@@ -23,63 +24,148 @@ namespace {
 constexpr int CHUNK = 2048;         // elements per table chunk: 8 per thread, loads of a chunk in flight together
 constexpr int QBLOCK = 256;         // elements per 8-bit scale: one wave, four consecutive elements per lane
 
+struct Coef {                       // what a step needs to know of a tensor
+    float decay, step_size, inv_bc2, eps, clip;
+    uint32_t t;
+    uint32_t pad[2];
+};
+static_assert(sizeof(Coef) == 32, "sca_adamw_scratch_bytes");
+
 struct AdamWArgs {
     const sca_adamw_tensor* tensors;
     const sca_adamw_chunk* chunks;
+    Coef* coef;                     // [n_tensors]
     int n_chunks, n_tensors;
     const float* hyper;             // sca_begin_step's block, or null: the scalars below and the tensors' own steps
     float lr, eps;
     double beta1, beta2, log_beta1, log_beta2;
     float b1, b2, one_minus_b1, one_minus_b2;       // 1 - beta taken in 64 bits: 1.0f - 0.999f is off by 1.3e-5
     uint64_t seed;
-    unsigned* done;                 // 0 before and after every launch
 };
 
-struct Coef {
-    float decay, step_size, inv_bc2, eps, clip;
-    uint32_t t;
-};
-
-__device__ __forceinline__ Coef coefficients(const AdamWArgs& a, const sca_adamw_tensor& q) {
-    Coef c;
-    float lr, bc1, bc2s;
+__global__ __launch_bounds__(256) void adamw_begin_kernel(const AdamWArgs a) {
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    if (j >= a.n_tensors) return;
+    const sca_adamw_tensor q = a.tensors[j];
+    Coef c = {};
+    float lr = a.lr, bc1, bc2s;
     if (a.hyper) {
-        lr = a.hyper[1]; bc1 = a.hyper[2]; bc2s = a.hyper[3]; c.eps = a.hyper[4]; c.clip = a.hyper[5]; c.t = 0;
+        lr = a.hyper[1]; bc1 = a.hyper[2]; bc2s = a.hyper[3]; c.eps = a.hyper[4]; c.clip = a.hyper[5];
     } else {
-        const double t = (double)(*q.step + 1);
-        lr = a.lr;
-        bc1 = (float)-expm1(t * a.log_beta1);           // 1 - beta^t without the cancellation
-        bc2s = (float)sqrt(-expm1(t * a.log_beta2));
-        c.eps = a.eps; c.clip = 0.f; c.t = (uint32_t)(*q.step + 1);
+        const int64_t t = *q.step + 1;
+        *q.step = t;
+        bc1 = (float)-expm1((double)t * a.log_beta1);           // 1 - beta^t without the cancellation
+        bc2s = (float)sqrt(-expm1((double)t * a.log_beta2));
+        c.eps = a.eps;
+        c.t = (uint32_t)t;
     }
     c.decay = 1.0f - lr * q.weight_decay;
     c.step_size = lr / bc1;
     c.inv_bc2 = 1.0f / bc2s;
-    return c;
+    a.coef[j] = c;
 }
 
+// denom = sqrt(v) / sqrt(1 - b2^t) + eps.  v_sqrt_f32 and v_rcp_f32 are good to one unit in the last place where their
+// arguments are ordinary numbers; the exact sequences (some 25 instructions) are for what is near the denormal ones.
 __device__ __forceinline__ float updated(float p, float m, float v, const Coef& c) {
-    return fmaf(-c.step_size, m / fmaf(sqrtf(v), c.inv_bc2, c.eps), p * c.decay);
+    const float denom = fmaf(__builtin_amdgcn_sqrtf(v), c.inv_bc2, c.eps);
+    float q = m * __builtin_amdgcn_rcpf(denom);
+    if (!(denom > 1e-17f && denom < 1e30f)) q = m / fmaf(sqrtf(v), c.inv_bc2, c.eps);
+    return fmaf(-c.step_size, q, p * c.decay);
 }
 
-// The 256 values x[lane][4] of a wave on the grid of an 8-bit float with MANT fraction bits and exponent bias BIAS,
-// behind a power of two: the four codes of a lane, and the scale.  rnd: 16 random bits per element; of the two grid
-// neighbours the upper one is taken where the way from the lower one exceeds 1 - rnd / 65536.
-template <int MANT, int BIAS, bool LEAST>
+// ---- 32-bit states ------------------------------------------------------------------------------------------------------
+// 2 x 4 elements of a chunk: all loads first.  28 bytes and some 30 instructions an element (fp32): bound by memory.
+template <typename T>
+__device__ __forceinline__ void chunk32(const sca_adamw_tensor& q, long long i0, const Coef& c, const AdamWArgs& a) {
+    float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
+    int left[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const long long i = i0 + h * 1024, l = q.n - i;
+        left[h] = l >= 4 ? 4 : l > 0 ? (int)l : 0;
+        const T *p = (const T*)q.p + i, *g = (const T*)q.g + i;
+        const float *m = (const float*)q.m + i, *v = (const float*)q.v + i;
+        if (q.vec && left[h] == 4) {
+            load_vec<T, 4>(p, pv[h]); load_vec<T, 4>(g, gv[h]); load_vec<float, 4>(m, mv[h]); load_vec<float, 4>(v, vv[h]);
+        } else {
+            load_part<T, 4>(p, left[h], pv[h]); load_part<T, 4>(g, left[h], gv[h]);
+            load_part<float, 4>(m, left[h], mv[h]); load_part<float, 4>(v, left[h], vv[h]);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const long long i = i0 + h * 1024;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float gk = gv[h][k];
+            if (c.clip > 0.f) gk = fminf(fmaxf(gk, -c.clip), c.clip);
+            mv[h][k] = fmaf(a.b1, mv[h][k], a.one_minus_b1 * gk);
+            vv[h][k] = fmaf(a.b2, vv[h][k], a.one_minus_b2 * gk * gk);
+            pv[h][k] = updated(pv[h][k], mv[h][k], vv[h][k], c);
+        }
+        T* p = (T*)q.p + i;
+        float *m = (float*)q.m + i, *v = (float*)q.v + i;
+        if (q.vec && left[h] == 4) {
+            store_vec<T, 4>(p, pv[h]); store_vec<float, 4>(m, mv[h]); store_vec<float, 4>(v, vv[h]);
+        } else {
+            store_part<T, 4>(p, left[h], pv[h]); store_part<float, 4>(m, left[h], mv[h]);
+            store_part<float, 4>(v, left[h], vv[h]);
+        }
+    }
+}
+
+// ---- 8-bit states -------------------------------------------------------------------------------------------------------
+// Philox4x32-10 as in common.h, with one 32 x 32 -> 64 bit product per pair of halves.
+__device__ __forceinline__ Philox4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)b;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)a;
+        k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
+    }
+    return Philox4{c0, c1, c2, c3};
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    v = dpp_umax<0xB1>(v);
+    v = dpp_umax<0x4E>(v);
+    v = dpp_umax<0x141>(v);
+    v = dpp_umax<0x140>(v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int r = 0; r < 64; r += 16) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)v, r);
+        m = o > m ? o : m;
+    }
+    return m;
+}
+
+// The 256 values x[lane][4] of a wave on the grid of an 8-bit float with MANT fraction bits and exponent bias BIAS, behind a
+// power of two: the four codes of a lane, and the scale.  rnd: 16 random bits per element; of the two grid neighbours the
+// upper one is taken where the way from the lower one is at least 1 - rnd / 65536.  For a normal number that is an integer
+// addition to its bits in front of the cut; the numbers below 2^(1 - BIAS) scales, whose steps are of equal size, take a
+// branch of their own.
+template <int MANT, int BIAS, bool SIGNED>
 __device__ __forceinline__ uint32_t to_grid(const float (&x)[4], const uint32_t (&rnd)[4], float& scale) {
     constexpr int TOP = MANT == 3 ? 8 : 15;             // the largest value is 1.75 * 2^TOP
     constexpr int DROP = 23 - MANT;
-    uint32_t amax = 0;
+    uint32_t b[4], amax = 0, amin = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
-        amax = b > amax ? b : amax;                     // as integers: a NaN is above every number
+        b[i] = __float_as_uint(x[i]) & 0x7fffffffu;
+        amax = b[i] > amax ? b[i] : amax;               // as integers: a NaN is above every number
+        amin = b[i] < amin ? b[i] : amin;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t b = __shfl_xor(amax, o, 64);
-        amax = b > amax ? b : amax;
-    }
+    amax = wave_umax(amax);
     if (amax == 0u || amax >= 0x7f800000u) {            // nothing, or not finite (then all 256 are NaN from now on)
         scale = amax == 0u ? 0.f : __uint_as_float(0x7fc00000u);
         return 0u;
@@ -87,166 +173,154 @@ __device__ __forceinline__ uint32_t to_grid(const float (&x)[4], const uint32_t 
     int e = (int)(amax >> 23) - 127 - TOP + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
     e = e < -126 ? -126 : e;
     scale = __uint_as_float((uint32_t)(e + 127) << 23);
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    // code = ((bits of x / scale) + random bits) >> DROP, the exponent counted from the type's; dividing by 2^e is a
+    // subtraction from the exponent
+    const uint32_t shift = (uint32_t)(e + 127 - BIAS) << 23, normal = (uint32_t)(e + 128 - BIAS + 0) << 23;
+    uint32_t code[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) code[i] = (b[i] + (rnd[i] << (DROP - 16)) - shift) >> DROP;
+    if (e + 128 - BIAS <= 0 || amin < normal) {
+        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float t = __uint_as_float(b[i]) * inv;
+            if (t < __uint_as_float((uint32_t)(128 - BIAS) << 23)) {
+                const float f = t * __uint_as_float((uint32_t)(127 + BIAS - 1 + MANT + 16) << 23);
+                code[i] = ((uint32_t)(int)f + rnd[i]) >> 16;
+                if (!SIGNED && code[i] == 0u && b[i] != 0u) code[i] = 1u;       // a positive moment stays positive
+            } else {
+                code[i] = ((__float_as_uint(t) + (rnd[i] << (DROP - 16))) >> DROP) - ((127 - BIAS) << MANT);
+            }
+        }
+    }
     uint32_t out = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float t = fabsf(x[i]) * inv;
-        uint32_t code;
-        if (t < __uint_as_float((uint32_t)(128 - BIAS) << 23)) {        // below 2^(1 - BIAS): steps of equal size
-            const float f = t * __uint_as_float((uint32_t)(127 + BIAS - 1 + MANT + 16) << 23);
-            code = ((uint32_t)(int)f + rnd[i]) >> 16;
-        } else {
-            code = ((__float_as_uint(t) + (rnd[i] << (DROP - 16))) >> DROP) - ((127 - BIAS) << MANT);
-        }
-        if (LEAST && code == 0u && x[i] > 0.f) code = 1u;
-        if (!LEAST && code != 0u && x[i] < 0.f) code |= 0x80u;
-        out |= code << (8 * i);
+        if (SIGNED) code[i] |= code[i] ? __float_as_uint(x[i]) >> 24 & 0x80u : 0u;
+        out |= code[i] << (8 * i);
     }
     return out;
 }
 
+// 2 x 4 elements of a chunk, a block of 256 per wave and half.  10 bytes (bf16) and some 100 instructions an element, a
+// third of them for the random bits and as many for the two roundings: bound by arithmetic.
 template <typename T>
-__device__ __forceinline__ void step32(const sca_adamw_tensor& q, long long i, int left, const Coef& c,
-                                       const AdamWArgs& a) {
-    T* p = (T*)q.p + i;
-    const T* g = (const T*)q.g + i;
-    float *m = (float*)q.m + i, *v = (float*)q.v + i;
-    float pv[4], gv[4], mv[4], vv[4];
-    const bool whole = q.vec && left >= 4;
-    if (whole) {
-        load_vec<T, 4>(p, pv); load_vec<T, 4>(g, gv); load_vec<float, 4>(m, mv); load_vec<float, 4>(v, vv);
-    } else {
-        load_part<T, 4>(p, left, pv); load_part<T, 4>(g, left, gv); load_part<float, 4>(m, left, mv);
-        load_part<float, 4>(v, left, vv);
-    }
+__device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, const Coef& c, const AdamWArgs& a) {
+    float pv[2][4], gv[2][4], ms[2], vs[2];
+    uint32_t mq[2], vq[2];
+    int left[2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float gk = gv[k];
-        if (c.clip > 0.f) gk = fminf(fmaxf(gk, -c.clip), c.clip);
-        mv[k] = fmaf(a.b1, mv[k], a.one_minus_b1 * gk);
-        vv[k] = fmaf(a.b2, vv[k], a.one_minus_b2 * gk * gk);
-        pv[k] = updated(pv[k], mv[k], vv[k], c);
-    }
-    if (whole) {
-        store_vec<T, 4>(p, pv); store_vec<float, 4>(m, mv); store_vec<float, 4>(v, vv);
-    } else {
-        store_part<T, 4>(p, left, pv); store_part<float, 4>(m, left, mv); store_part<float, 4>(v, left, vv);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void step8(const sca_adamw_tensor& q, long long i, int left, const Coef& c, const AdamWArgs& a) {
-    T* p = (T*)q.p + i;
-    const T* g = (const T*)q.g + i;
-    uint8_t *m = (uint8_t*)q.m + i, *v = (uint8_t*)q.v + i;
-    const long long blk = i / QBLOCK;
-    float pv[4], gv[4], mn[4], vn[4];
-    uint32_t mq = 0, vq = 0;
-    const bool whole = q.vec && left >= 4;
-    if (whole) {
-        load_vec<T, 4>(p, pv); load_vec<T, 4>(g, gv);
-        mq = *(const uint32_t*)m; vq = *(const uint32_t*)v;
-    } else {
-        load_part<T, 4>(p, left, pv); load_part<T, 4>(g, left, gv);
-        for (int k = 0; k < 4; ++k)
-            if (k < left) {
-                mq |= (uint32_t)m[k] << (8 * k);
-                vq |= (uint32_t)v[k] << (8 * k);
-            }
-    }
-    // (a wave whose block lies behind the tensor's end has nothing to do; the scale of its block does not exist)
-    const bool any = (i & ~(long long)(QBLOCK - 1)) < q.n;
-    const double ms = any ? (double)q.m_scale[blk] : 0.0, vs = any ? (double)q.v_scale[blk] : 0.0;
-    const float md[4] = {__builtin_amdgcn_cvt_f32_fp8((int)mq, 0), __builtin_amdgcn_cvt_f32_fp8((int)mq, 1),
-                         __builtin_amdgcn_cvt_f32_fp8((int)mq, 2), __builtin_amdgcn_cvt_f32_fp8((int)mq, 3)};
-    const float vd[4] = {__builtin_amdgcn_cvt_f32_bf8((int)vq, 0), __builtin_amdgcn_cvt_f32_bf8((int)vq, 1),
-                         __builtin_amdgcn_cvt_f32_bf8((int)vq, 2), __builtin_amdgcn_cvt_f32_bf8((int)vq, 3)};
+    for (int h = 0; h < 2; ++h) {
+        const long long i = i0 + h * 1024, l = q.n - i;
+        left[h] = l >= 4 ? 4 : l > 0 ? (int)l : 0;
+        const T *p = (const T*)q.p + i, *g = (const T*)q.g + i;
+        const uint8_t *m = (const uint8_t*)q.m + i, *v = (const uint8_t*)q.v + i;
+        // (a wave whose block lies behind the tensor's end has nothing to do, and there is no scale of its block)
+        const bool any = (i & ~(long long)(QBLOCK - 1)) < q.n;
+        ms[h] = any ? q.m_scale[i / QBLOCK] : 0.f;
+        vs[h] = any ? q.v_scale[i / QBLOCK] : 0.f;
+        if (q.vec && left[h] == 4) {
+            load_vec<T, 4>(p, pv[h]); load_vec<T, 4>(g, gv[h]);
+            mq[h] = *(const uint32_t*)m; vq[h] = *(const uint32_t*)v;
+        } else {
+            load_part<T, 4>(p, left[h], pv[h]); load_part<T, 4>(g, left[h], gv[h]);
+            mq[h] = vq[h] = 0u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const double gd = (double)gv[k];
-        mn[k] = k < left ? (float)fma(a.beta1, (double)md[k] * ms, (1.0 - a.beta1) * gd) : 0.f;
-        vn[k] = k < left ? (float)fma(a.beta2, (double)vd[k] * vs, (1.0 - a.beta2) * gd * gd) : 0.f;
-        pv[k] = updated(pv[k], mn[k], vn[k], c);
-    }
-    const Philox4 w = philox4x32_10((uint32_t)(i >> 2), (uint32_t)((unsigned long long)i >> 34), (uint32_t)q.id, c.t,
-                                    (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
-    const uint32_t wm[4] = {w.x & 0xffffu, w.y & 0xffffu, w.z & 0xffffu, w.w & 0xffffu};
-    const uint32_t wv[4] = {w.x >> 16, w.y >> 16, w.z >> 16, w.w >> 16};
-    float msn, vsn;
-    mq = to_grid<3, 7, false>(mn, wm, msn);
-    vq = to_grid<2, 15, true>(vn, wv, vsn);
-    if (!any) return;
-    if (whole) {
-        store_vec<T, 4>(p, pv);
-        *(uint32_t*)m = mq; *(uint32_t*)v = vq;
-    } else {
-        store_part<T, 4>(p, left, pv);
-        for (int k = 0; k < 4; ++k)
-            if (k < left) {
-                m[k] = (uint8_t)(mq >> (8 * k));
-                v[k] = (uint8_t)(vq >> (8 * k));
-            }
-    }
-    if ((threadIdx.x & 63) == 0) {
-        q.m_scale[blk] = msn;
-        q.v_scale[blk] = vsn;
-    }
-}
-
-template <int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(const AdamWArgs a) {
-    for (int k = blockIdx.x; k < a.n_chunks; k += gridDim.x) {
-        const sca_adamw_chunk ch = a.chunks[k];
-        const sca_adamw_tensor q = a.tensors[ch.tensor];
-        const Coef c = coefficients(a, q);
-        for (int h = 0; h < CHUNK; h += 1024) {
-            const long long i = (long long)ch.index * CHUNK + h + 4 * threadIdx.x;
-            const long long l = q.n - i;
-            const int left = l >= 4 ? 4 : l > 0 ? (int)l : 0;
-            if (BITS == 32) {
-                if (left <= 0) continue;
-                if (q.dtype == SCA_F32) step32<float>(q, i, left, c, a);
-                else if (q.dtype == SCA_BF16) step32<sca_bf16>(q, i, left, c, a);
-                else step32<sca_f16>(q, i, left, c, a);
-            } else {
-                if (q.dtype == SCA_F32) step8<float>(q, i, left, c, a);
-                else if (q.dtype == SCA_BF16) step8<sca_bf16>(q, i, left, c, a);
-                else step8<sca_f16>(q, i, left, c, a);
-            }
+            for (int k = 0; k < 4; ++k)
+                if (k < left[h]) {
+                    mq[h] |= (uint32_t)m[k] << (8 * k);
+                    vq[h] |= (uint32_t)v[k] << (8 * k);
+                }
         }
     }
-    if (a.hyper) return;
-    // every workgroup has read the steps it needs before it counts itself done; the last one advances them
-    __shared__ unsigned last;
-    __syncthreads();
-    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (last != gridDim.x - 1) return;
-    for (int j = threadIdx.x; j < a.n_tensors; j += 256) *a.tensors[j].step += 1;
-    if (threadIdx.x == 0) *a.done = 0u;
+    const double one_b1 = 1.0 - a.beta1, one_b2 = 1.0 - a.beta2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const long long i = i0 + h * 1024;
+        if ((i & ~(long long)(QBLOCK - 1)) >= q.n) return;
+        const double bm = a.beta1 * (double)ms[h], bv = a.beta2 * (double)vs[h];
+        const float md[4] = {__builtin_amdgcn_cvt_f32_fp8((int)mq[h], 0), __builtin_amdgcn_cvt_f32_fp8((int)mq[h], 1),
+                             __builtin_amdgcn_cvt_f32_fp8((int)mq[h], 2), __builtin_amdgcn_cvt_f32_fp8((int)mq[h], 3)};
+        const float vd[4] = {__builtin_amdgcn_cvt_f32_bf8((int)vq[h], 0), __builtin_amdgcn_cvt_f32_bf8((int)vq[h], 1),
+                             __builtin_amdgcn_cvt_f32_bf8((int)vq[h], 2), __builtin_amdgcn_cvt_f32_bf8((int)vq[h], 3)};
+        float mn[4], vn[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double gd = (double)gv[h][k];
+            mn[k] = (float)fma((double)md[k], bm, one_b1 * gd);
+            vn[k] = (float)fma(one_b2 * gd, gd, (double)vd[k] * bv);
+            if (left[h] < 4 && k >= left[h]) mn[k] = vn[k] = 0.f;       // (behind the end; a NaN scale must not get in)
+            pv[h][k] = updated(pv[h][k], mn[k], vn[k], c);
+        }
+        const Philox4 w = philox((uint32_t)(i >> 2), (uint32_t)((unsigned long long)i >> 34), (uint32_t)q.id, c.t,
+                                 (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
+        const uint32_t wm[4] = {w.x & 0xffffu, w.y & 0xffffu, w.z & 0xffffu, w.w & 0xffffu};
+        const uint32_t wv[4] = {w.x >> 16, w.y >> 16, w.z >> 16, w.w >> 16};
+        float msn, vsn;
+        const uint32_t mc = to_grid<3, 7, true>(mn, wm, msn), vc = to_grid<2, 15, false>(vn, wv, vsn);
+        T* p = (T*)q.p + i;
+        uint8_t *m = (uint8_t*)q.m + i, *v = (uint8_t*)q.v + i;
+        if (q.vec && left[h] == 4) {
+            store_vec<T, 4>(p, pv[h]);
+            *(uint32_t*)m = mc; *(uint32_t*)v = vc;
+        } else {
+            store_part<T, 4>(p, left[h], pv[h]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < left[h]) {
+                    m[k] = (uint8_t)(mc >> (8 * k));
+                    v[k] = (uint8_t)(vc >> (8 * k));
+                }
+        }
+        if ((threadIdx.x & 63) == 0) {
+            q.m_scale[i / QBLOCK] = msn;
+            q.v_scale[i / QBLOCK] = vsn;
+        }
+    }
+}
+
+// One chunk per workgroup.  (As many workgroups as fit, each walking every so many chunks, take 20 % longer: they do not
+// end together.)
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamWArgs a) {
+    for (long long k = blockIdx.x; k < a.n_chunks; k += gridDim.x) {
+        const sca_adamw_chunk ch = a.chunks[k];
+        const sca_adamw_tensor q = a.tensors[ch.tensor];
+        const Coef c = a.coef[ch.tensor];
+        const long long i = (long long)ch.index * CHUNK + 4 * threadIdx.x;
+        if (BITS == 32) {
+            if (q.dtype == SCA_F32) chunk32<float>(q, i, c, a);
+            else if (q.dtype == SCA_BF16) chunk32<sca_bf16>(q, i, c, a);
+            else chunk32<sca_f16>(q, i, c, a);
+        } else {
+            if (q.dtype == SCA_F32) chunk8<float>(q, i, c, a);
+            else if (q.dtype == SCA_BF16) chunk8<sca_bf16>(q, i, c, a);
+            else chunk8<sca_f16>(q, i, c, a);
+        }
+    }
 }
 
 }  // namespace
 
 extern "C" int sca_adamw_chunk_elements(void) { return CHUNK; }
 extern "C" int sca_adamw_block_elements(void) { return QBLOCK; }
+extern "C" long long sca_adamw_scratch_bytes(int n_tensors) { return n_tensors < 0 ? -1 : (long long)n_tensors * sizeof(Coef); }
 
 extern "C" int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_adamw_chunk* chunks,
                               int n_chunks, int state_bits, const float* hyper, float lr, double beta1, double beta2,
-                              float eps, uint64_t seed, uint32_t* done, void* stream) {
+                              float eps, uint64_t seed, void* scratch, void* stream) {
     if (n_tensors < 0 || n_chunks < 0 || (state_bits != 32 && state_bits != 8)) return -1;
     if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return -1;
-    if (!hyper && !(eps >= 0.f && done)) return -1;
-    if (hyper && state_bits != 32) return -1;
+    if (hyper ? state_bits != 32 : !(eps >= 0.f)) return -1;
     if (n_tensors == 0) return 0;
-    if (!tensors || (n_chunks > 0 && !chunks)) return -1;
-    AdamWArgs a{tensors, chunks, n_chunks, n_tensors, hyper, lr, eps, beta1, beta2, log(beta1), log(beta2),
-                (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), seed, (unsigned*)done};
-    int grid = n_chunks < 2048 ? n_chunks : 2048;
-    if (grid < 1) grid = 1;
-    if (state_bits == 32) hipLaunchKernelGGL((adamw_kernel<32>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((adamw_kernel<8>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+    if (!tensors || !scratch || ((uintptr_t)scratch & 15) || (n_chunks > 0 && !chunks)) return -1;
+    hipStream_t st = (hipStream_t)stream;
+    const AdamWArgs a{tensors, chunks, (Coef*)scratch, n_chunks, n_tensors, hyper, lr, eps, beta1, beta2, log(beta1),
+                      log(beta2), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), seed};
+    hipLaunchKernelGGL(adamw_begin_kernel, dim3((n_tensors + 255) / 256), dim3(256), 0, st, a);
+    const int grid = n_chunks < (1 << 23) ? n_chunks : 1 << 23;         // fewer than 2^32 threads
+    if (grid > 0 && state_bits == 32) hipLaunchKernelGGL((adamw_kernel<32>), dim3(grid), dim3(256), 0, st, a);
+    else if (grid > 0) hipLaunchKernelGGL((adamw_kernel<8>), dim3(grid), dim3(256), 0, st, a);
     SCA_CHECK_LAUNCH();
     return 0;
 }

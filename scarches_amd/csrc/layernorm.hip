@@ -147,15 +147,12 @@ struct LnBwd {
     float* part;                 // [slab][2][n] partial sums of (dw, db), or null
 };
 
-// Threads of a workgroup: eight waves of rows of up to 64 threads each, or one row.
-template <int TPR>
-constexpr int bwd_threads() { return TPR > 64 ? TPR : 512; }
-
-template <typename T, typename W, int TPR, int V, int MODE>
-__global__ __launch_bounds__(bwd_threads<TPR>()) void ln_bwd_kernel(const LnBwd a) {
-    constexpr int VEC = vec_of<T>(), NT = bwd_threads<TPR>(), PER = NT / TPR;
+// NT threads, TPR of them a row.
+template <typename T, typename W, int TPR, int V, int MODE, int NT>
+__global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
+    constexpr int VEC = vec_of<T>(), PER = NT / TPR, COLS = TPR * V * VEC;
     __shared__ float scratch[16];
-    __shared__ float sums[TPR > 64 ? 1 : 2 * TPR * V * VEC];     // (one row per workgroup: nothing to add up)
+    __shared__ __attribute__((aligned(16))) float sums[PER > 1 ? PER * COLS : 4];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, n = a.n;
     const float inv_n = 1.f / (float)n;
     float g[V][VEC], dw[V][VEC], db[V][VEC];
@@ -166,9 +163,11 @@ __global__ __launch_bounds__(bwd_threads<TPR>()) void ln_bwd_kernel(const LnBwd 
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dw[j][i] = db[j][i] = 0.f;
     }
-    for (long long r = (long long)blockIdx.x * PER + sub; r < a.rows; r += (long long)gridDim.x * PER) {
+    const long long step = (long long)gridDim.x * PER;
+    raw_t xq[V] = {}, dq[V] = {};
+    float mean = 0.f, rstd = 0.f;
+    auto load = [&](long long r) {
         const T *xr = (const T*)a.x + r * a.ldx, *dr = (const T*)a.dy + r * a.lddy;
-        raw_t xq[V] = {}, dq[V] = {};
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const Cols<T, TPR, MODE> at(j, t, n);
@@ -177,17 +176,34 @@ __global__ __launch_bounds__(bwd_threads<TPR>()) void ln_bwd_kernel(const LnBwd 
                 load_cols<MODE>(dr, at.c, n, dq[j]);
             }
         }
-        const float mean = a.stats[r], rstd = a.stats[a.rows + r];
+        mean = a.stats[r];
+        rstd = a.stats[a.rows + r];
+    };
+    // 16-bit rows, whose arithmetic takes half as long as their loads: the next row is on its way meanwhile (16384 x 4000
+    // bf16: 81 instead of 100 us).  fp32 rows have no registers for it and run at the rate of a copy without.
+    constexpr bool AHEAD = sizeof(T) == 2;
+    long long r = (long long)blockIdx.x * PER + sub;
+    if (AHEAD && r < a.rows) load(r);
+    for (; r < a.rows; r += step) {
+        if (!AHEAD) load(r);
+        raw_t x0[V], d0[V];
+        const float mean0 = mean, rstd0 = rstd;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            x0[j] = xq[j];
+            d0[j] = dq[j];
+        }
+        if (AHEAD && r + step < a.rows) load(r + step);
         float s1 = 0.f, s2 = 0.f, h[VEC], d[VEC];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const Cols<T, TPR, MODE> at(j, t, n);
             if (!at.there) continue;
-            unpack<T>(xq[j], h);
-            unpack<T>(dq[j], d);
+            unpack<T>(x0[j], h);
+            unpack<T>(d0[j], d);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                h[i] = (h[i] - mean) * rstd;
+                h[i] = (h[i] - mean0) * rstd0;
                 dw[j][i] = fmaf(d[i], h[i], dw[j][i]);
                 db[j][i] += d[i];
                 const float p = at.own(i, n) ? d[i] * g[j][i] : 0.f;
@@ -202,58 +218,40 @@ __global__ __launch_bounds__(bwd_threads<TPR>()) void ln_bwd_kernel(const LnBwd 
         for (int j = 0; j < V; ++j) {
             const Cols<T, TPR, MODE> at(j, t, n);
             if (!at.there) continue;
-            unpack_again<T>(xq[j], h);
-            unpack_again<T>(dq[j], d);
+            unpack_again<T>(x0[j], h);
+            unpack_again<T>(d0[j], d);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) d[i] = rstd * (fmaf(d[i], g[j][i], -m1) - (h[i] - mean) * rstd * m2);
+            for (int i = 0; i < VEC; ++i) d[i] = rstd0 * (fmaf(d[i], g[j][i], -m1) - (h[i] - mean0) * rstd0 * m2);
             store_cols<MODE>(out, at.c, n, d);
         }
     }
     if (!a.part) return;
     float* slab = a.part + (long long)blockIdx.x * 2 * n;
-    if constexpr (TPR > 64) {
+    auto put = [&](const float (&v)[V][VEC], float* out) {
+        if constexpr (PER == 1) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const Cols<T, TPR, MODE> at(j, t, n);
-            if (!at.there) continue;
-            store_vec<float, VEC>(slab + at.c, dw[j]);
-            store_vec<float, VEC>(slab + n + at.c, db[j]);
-        }
-    } else {
-        // the workgroup's rows one after the other into LDS (vectors, columns as the threads hold them)
-        for (int k = 0; k < PER; ++k) {
+            for (int j = 0; j < V; ++j) {
+                const Cols<T, TPR, MODE> at(j, t, n);
+                if (at.there) store_vec<float, VEC>(out + at.c, v[j]);
+            }
+        } else {
+            // the rows' sums side by side in LDS, each column added up by one thread
             __syncthreads();
-            if (sub != k) continue;
 #pragma unroll
-            for (int j = 0; j < V; ++j)
+            for (int j = 0; j < V; ++j) store_vec<float, VEC>(sums + sub * COLS + (j * TPR + t) * VEC, v[j]);
+            __syncthreads();
+            for (int o = threadIdx.x; o < COLS; o += NT) {
+                const int first = o / VEC * VEC, i = o % VEC;
+                if (first >= n || (MODE == ROW_TINY && i >= n)) continue;
+                float s = 0.f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int o = (j * VEC + i) * TPR + t;
-                    sums[o] = k ? sums[o] + dw[j][i] : dw[j][i];
-                    sums[TPR * V * VEC + o] = k ? sums[TPR * V * VEC + o] + db[j][i] : db[j][i];
-                }
-        }
-        __syncthreads();
-        if (sub) return;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const Cols<T, TPR, MODE> at(j, t, n);
-            if (!at.there) continue;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int o = (j * VEC + i) * TPR + t;
-                dw[j][i] = sums[o];
-                db[j][i] = sums[TPR * V * VEC + o];
-            }
-            if (MODE == ROW_TINY) {
-                store_part<float, VEC>(slab, n, dw[j]);
-                store_part<float, VEC>(slab + n, n, db[j]);
-            } else {
-                store_vec<float, VEC>(slab + at.c, dw[j]);
-                store_vec<float, VEC>(slab + n + at.c, db[j]);
+                for (int k = 0; k < PER; ++k) s += sums[k * COLS + o];
+                out[(MODE == ROW_RAGGED && first > n - VEC ? n - VEC : first) + i] = s;
             }
         }
-    }
+    };
+    put(dw, slab);
+    put(db, slab + n);
 }
 
 // Rows beyond the registers: one workgroup per row for dx, and columns by slabs of rows for dw and db.
@@ -305,22 +303,24 @@ __global__ __launch_bounds__(256) void ln_dw_long_kernel(const LnBwd a) {
     a.part[(long long)blockIdx.x * 2 * a.n + a.n + c] = sb;
 }
 
-// dw and db from the slabs: 64 columns per workgroup, 16 threads a column, added in a fixed order.
+// dw and db from the slabs: 32 columns per workgroup, 32 threads a column, added in a fixed order.
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restrict__ part, int slabs, int n,
                                                             W* __restrict__ dw, W* __restrict__ db) {
-    __shared__ float sum[16][64];
-    const int lane = threadIdx.x & 63, k = threadIdx.x >> 6;
-    const long long c = (long long)blockIdx.x * 64 + lane;       // column of [dw | db]
+    __shared__ float sum[32][33];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const long long c = (long long)blockIdx.x * 32 + lane, width = 2LL * n;      // column of [dw | db]
     float v = 0.f;
-    if (c < 2LL * n)
-        for (int s = k; s < slabs; s += 16) v += part[(long long)s * 2 * n + c];
+    if (c < width) {
+#pragma unroll 8
+        for (int s = k; s < slabs; s += 32) v += part[s * width + c];
+    }
     sum[k][lane] = v;
     __syncthreads();
-    if (k || c >= 2LL * n) return;
+    if (k || c >= width) return;
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v += sum[i][lane];
+    for (int i = 0; i < 32; ++i) v += sum[i][lane];
     W* out = c < n ? dw : db;
     if (out) out[c < n ? c : c - n] = from_f32<W>(v);
 }
@@ -328,15 +328,16 @@ __global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restr
 // ---- launches ---------------------------------------------------------------------------------------------------------
 constexpr int CUS = 256;
 
-// How a row of `vecs` vectors is held: TPR threads, V vectors each (the backward pass keeps five values per element).
-// Slabs of partial sums of the weight gradients: one workgroup per CU walks the rows, as many workgroups as there are rows
-// to fill them.
-struct BwdShape { int tpr, slabs; };
+// How the backward pass holds a row of `vecs` vectors: TPR threads, at most 32 elements each (five values are kept per
+// element); 0: not at all.  nt: threads of a workgroup - half as many where there are not enough rows to give every CU
+// eight waves.  slabs: one slab of partial sums per workgroup, which walks the rows: one workgroup per CU.
+struct BwdShape { int tpr, nt, slabs; };
 BwdShape bwd_shape(long long rows, int n, int vec) {
     const int vecs = (n + vec - 1) / vec, v = 32 / vec;
     BwdShape s;
-    s.tpr = vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 * v ? 64 : vecs <= 256 * v ? 256 : n <= 16384 ? 1024 : 0;
-    const int per = s.tpr == 0 ? 1 : s.tpr > 64 ? 1 : 512 / s.tpr;
+    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 * v ? 64 : vecs <= 256 * v ? 256 : n <= 16384 ? 1024 : 0;
+    s.nt = s.tpr > 64 ? s.tpr : rows * s.tpr <= 512 * CUS ? 256 : 512;
+    const int per = s.tpr == 0 ? 1 : s.nt / s.tpr;
     const long long blocks = (rows + per - 1) / per;
     const int most = s.tpr == 256 ? 2 * CUS : CUS;
     s.slabs = (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
@@ -360,10 +361,11 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
     } while (0)
     if (mode == ROW_TINY) {
         constexpr int NT = 256;
-        const long long blocks = (rows + 15) / 16;
-        FWD_MODE(16, 1, ROW_TINY);
+        const long long blocks = (rows + 63) / 64;
+        FWD_MODE(4, 1, ROW_TINY);
     }
     // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory.
+    else if (vecs <= 4) FWD(4, 1);
     else if (vecs <= 16) FWD(16, 1);
     else if (vecs <= 32) FWD(32, 1);
     else if (vecs <= 64) FWD(64, 1);
@@ -391,22 +393,30 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
     const int n = a.n, vecs = (n + VEC - 1) / VEC, mode = row_mode(n, VEC);
     const BwdShape sh = bwd_shape(a.rows, n, VEC);
     if (a.rows > 0 && sh.tpr) {
-#define BWD_MODE(TPR, V, MODE)                                                                                            \
-    hipLaunchKernelGGL((ln_bwd_kernel<T, W, TPR, V, MODE>), dim3((unsigned)grid), dim3(bwd_threads<TPR>()), 0, st, a)
-#define BWD(TPR, V)                                         \
-    do {                                                    \
-        if (mode == ROW_FULL) BWD_MODE(TPR, V, ROW_FULL);   \
-        else BWD_MODE(TPR, V, ROW_RAGGED);                  \
+#define BWD_MODE(TPR, V, MODE, NT)                                                                                        \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, W, TPR, V, MODE, NT>), dim3((unsigned)sh.slabs), dim3(NT), 0, st, a)
+#define BWD(TPR, V, NT)                                         \
+    do {                                                        \
+        if (mode == ROW_FULL) BWD_MODE(TPR, V, ROW_FULL, NT);   \
+        else BWD_MODE(TPR, V, ROW_RAGGED, NT);                  \
     } while (0)
-        const int grid = sh.slabs;
-        if (mode == ROW_TINY) BWD_MODE(16, 1, ROW_TINY);
-        else if (vecs <= 16) BWD(16, 1);
-        else if (vecs <= 32) BWD(32, 1);
-        else if (vecs <= 64) BWD(64, 1);
-        else if (V > 4 && vecs <= 64 * 4) BWD(64, (V > 4 ? 4 : V));
-        else if (vecs <= 64 * V) BWD(64, V);
-        else if (vecs <= 256 * V) BWD(256, V);
-        else BWD(1024, V / 2);
+#define BWD2(TPR, V)                        \
+    do {                                    \
+        if (sh.nt == 256) BWD(TPR, V, 256); \
+        else BWD(TPR, V, 512);              \
+    } while (0)
+        if (mode == ROW_TINY && sh.nt == 256) BWD_MODE(4, 1, ROW_TINY, 256);
+        else if (mode == ROW_TINY) BWD_MODE(4, 1, ROW_TINY, 512);
+        else if (vecs <= 4) BWD2(4, 1);
+        else if (vecs <= 16) BWD2(16, 1);
+        else if (vecs <= 32) BWD2(32, 1);
+        else if (vecs <= 64) BWD2(64, 1);
+        else if (vecs <= 64 * 2) BWD2(64, 2);
+        else if (V > 4 && vecs <= 64 * 4) BWD2(64, (V > 4 ? 4 : V));
+        else if (vecs <= 64 * V) BWD2(64, V);
+        else if (vecs <= 256 * V) BWD(256, V, 256);
+        else BWD(1024, V / 2, 1024);
+#undef BWD2
 #undef BWD
 #undef BWD_MODE
     } else if (a.rows > 0) {
@@ -415,7 +425,7 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
             hipLaunchKernelGGL((ln_dw_long_kernel<T>), dim3(sh.slabs, (n + 255) / 256), dim3(256), 0, st, a);
     }
     if (dw || db)
-        hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((unsigned)((2LL * n + 63) / 64)), dim3(1024), 0, st, a.part,
+        hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((unsigned)((2LL * n + 31) / 32)), dim3(1024), 0, st, a.part,
                            a.rows > 0 ? sh.slabs : 0, n, (W*)dw, (W*)db);
     SCA_CHECK_LAUNCH();
     return 0;

@@ -91,10 +91,13 @@ __device__ __forceinline__ void store_cols(T* __restrict__ row, int c, int n, co
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* scratch) {
     if constexpr (TPR >= 64) v = wave_sum(v);
-    else {
+    else if constexpr (TPR == 4) {
+        v += dpp_f32<0xB1>(v);      // quad_perm [1,0,3,2]
+        v += dpp_f32<0x4E>(v);      // quad_perm [2,3,0,1]
+    } else {
         v = row16_sum(v);
         if constexpr (TPR == 32) v += __shfl_xor(v, 16, 64);
-        static_assert(TPR >= 16, "rows of 16 lanes and more");
+        static_assert(TPR >= 16, "rows of 4, 16, 32, 64 or more lanes");
     }
     if constexpr (TPR > 64) {
         __syncthreads();

@@ -274,7 +274,7 @@ def _dense(t):
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW (decoupled weight decay) over all parameters of a group in one launch.
+    """torch.optim.AdamW (decoupled weight decay) over all parameters of a group at once.
 
     params, lr, betas, eps, weight_decay: as torch.optim.AdamW.  Parameters are float32, bfloat16 or float16; a step is
     computed in float32 and rounded once.
@@ -305,7 +305,7 @@ class AdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, not {state_bits}")
         self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFFFFFFFFFF
-        self._steps = {}            # group number -> int64 [parameters + 1] on the device: their steps, the kernel's counter
+        self._steps = {}            # group number -> int64 [parameters] on the device: their steps
         self._plans = {}            # group number -> the table of the last step()
         self._captured = []         # tables (and what they point to) that captured graphs read
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -341,13 +341,13 @@ class AdamW(torch.optim.Optimizer):
         ctr = self._steps.get(gi)
         params = self.param_groups[gi]["params"]
         if ctr is None:
-            ctr = self._steps[gi] = torch.zeros(len(params) + 1, dtype=torch.int64, device=params[0].device)
+            ctr = self._steps[gi] = torch.zeros(len(params), dtype=torch.int64, device=params[0].device)
         return ctr
 
     def set_step(self, step: int):
         """Set the number of steps that every parameter has behind it (a run taken up from states of another program)."""
         for gi in range(len(self.param_groups)):
-            self._group_steps(gi)[:-1].fill_(int(step))
+            self._group_steps(gi).fill_(int(step))
 
     def state_dict(self):
         """torch's layout; every parameter's state has `step` as a whole number (read from the device)."""
@@ -377,7 +377,7 @@ class AdamW(torch.optim.Optimizer):
                 if st:      # the types of the states are theirs, not the parameter's
                     self.state[p] = {k: st[k].to(p.device, torch.float32 if self.state_bits == 32 else st[k].dtype,
                                                  copy=True) for k in keys}
-            self._group_steps(gi)[:-1].copy_(torch.tensor(steps))
+            self._group_steps(gi).copy_(torch.tensor(steps))
 
     # ------------------------------------------------------------------------------------------ step
     def _table(self, gi, group, key):
@@ -424,12 +424,14 @@ class AdamW(torch.optim.Optimizer):
         chunks[:, 0] = np.repeat(np.arange(len(rows)), counts)
         chunks[:, 1] = np.arange(len(chunks)) - np.repeat(np.cumsum(counts) - counts, counts)
         entries = bytes((_lib.AdamWTensor * len(rows))(*rows))
-        # one pinned block, one copy on the current stream (the caching host allocator keeps the block until it has run)
-        host = torch.from_numpy(np.frombuffer(entries + chunks.tobytes(), dtype=np.uint8).copy()).pin_memory()
+        # one pinned block, one copy on the current stream (the caching host allocator keeps the block until it has run);
+        # the kernels' scratch comes first, where the block's alignment is
+        size = lib.sca_adamw_scratch_bytes(len(rows))
+        host = torch.from_numpy(np.frombuffer(bytes(size) + entries + chunks.tobytes(), dtype=np.uint8).copy()).pin_memory()
         table = host.to(dev, non_blocking=True)
-        at = table.data_ptr()
+        at = table.data_ptr() + size
         return dict(key=key, table=table, streams={torch.cuda.current_stream(dev).cuda_stream}, entries=at, n=len(rows), chunks=at + len(entries), n_chunks=len(chunks),
-                    steps=steps, done=steps.data_ptr() + 8 * len(group["params"]), device=dev)
+                    steps=steps, scratch=table.data_ptr(), device=dev)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -465,5 +467,5 @@ class AdamW(torch.optim.Optimizer):
                     plan["table"].record_stream(stream)
             b1, b2 = group["betas"]
             _call(plan["device"], "sca_adamw_step", plan["entries"], plan["n"], plan["chunks"], plan["n_chunks"],
-                  self.state_bits, None, float(group["lr"]), b1, b2, float(group["eps"]), self.seed, plan["done"])
+                  self.state_bits, None, float(group["lr"]), b1, b2, float(group["eps"]), self.seed, plan["scratch"])
         return loss
