@@ -65,13 +65,24 @@ __global__ __launch_bounds__(256) void adamw_begin_kernel(const AdamWArgs a) {
     a.coef[j] = c;
 }
 
-// denom = sqrt(v) / sqrt(1 - b2^t) + eps.  v_sqrt_f32 and v_rcp_f32 are good to one unit in the last place where their
-// arguments are ordinary numbers; the exact sequences (some 25 instructions) are for what is near the denormal ones.
-__device__ __forceinline__ float updated(float p, float m, float v, const Coef& c) {
-    const float denom = fmaf(__builtin_amdgcn_sqrtf(v), c.inv_bc2, c.eps);
-    float q = m * __builtin_amdgcn_rcpf(denom);
-    if (!(denom > 1e-17f && denom < 1e30f)) q = m / fmaf(sqrtf(v), c.inv_bc2, c.eps);
-    return fmaf(-c.step_size, q, p * c.decay);
+// p of four elements.  denom = sqrt(v) / sqrt(1 - b2^t) + eps; v_sqrt_f32 and v_rcp_f32 are good to one unit in the last
+// place where their arguments are ordinary numbers, the exact sequences (some 25 instructions) are for what is near the
+// denormal ones.
+__device__ __forceinline__ void update(float (&p)[4], const float (&m)[4], const float (&v)[4], const Coef& c) {
+    float denom[4], q[4], lo = 1e30f, hi = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        denom[k] = fmaf(__builtin_amdgcn_sqrtf(v[k]), c.inv_bc2, c.eps);
+        q[k] = m[k] * __builtin_amdgcn_rcpf(denom[k]);
+        lo = fminf(lo, denom[k]);
+        hi = fmaxf(hi, denom[k]);
+    }
+    if (!(lo > 1e-17f && hi < 1e30f)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = m[k] / fmaf(sqrtf(v[k]), c.inv_bc2, c.eps);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = fmaf(-c.step_size, q[k], p[k] * c.decay);
 }
 
 // ---- 32-bit states ------------------------------------------------------------------------------------------------------
@@ -102,8 +113,8 @@ __device__ __forceinline__ void chunk32(const sca_adamw_tensor& q, long long i0,
             if (c.clip > 0.f) gk = fminf(fmaxf(gk, -c.clip), c.clip);
             mv[h][k] = fmaf(a.b1, mv[h][k], a.one_minus_b1 * gk);
             vv[h][k] = fmaf(a.b2, vv[h][k], a.one_minus_b2 * gk * gk);
-            pv[h][k] = updated(pv[h][k], mv[h][k], vv[h][k], c);
         }
+        update(pv[h], mv[h], vv[h], c);
         T* p = (T*)q.p + i;
         float *m = (float*)q.m + i, *v = (float*)q.v + i;
         if (q.vec && left[h] == 4) {
@@ -121,9 +132,9 @@ __device__ __forceinline__ Philox4 philox(uint32_t c0, uint32_t c1, uint32_t c2,
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(b >> 32), c1, k0, 0x96);       // a ^ b ^ c
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(a >> 32), c3, k1, 0x96);
         c3 = (uint32_t)a;
         k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
     }
@@ -150,18 +161,18 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 }
 
 // The 256 values x[lane][4] of a wave on the grid of an 8-bit float with MANT fraction bits and exponent bias BIAS, behind a
-// power of two: the four codes of a lane, and the scale.  rnd: 16 random bits per element; of the two grid neighbours the
-// upper one is taken where the way from the lower one is at least 1 - rnd / 65536.  For a normal number that is an integer
-// addition to its bits in front of the cut; the numbers below 2^(1 - BIAS) scales, whose steps are of equal size, take a
-// branch of their own.
+// power of two: the four codes of a lane, and the scale.  w: a random word per element, whose low (SIGNED: the first
+// moment) or high half decides: of the two grid neighbours the upper one is taken where the way from the lower one is at
+// least 1 - half / 65536.  For a normal number that is an integer addition to its bits in front of the cut; the numbers
+// below 2^(1 - BIAS) scales, whose steps are of equal size, take a branch of their own.
 template <int MANT, int BIAS, bool SIGNED>
-__device__ __forceinline__ uint32_t to_grid(const float (&x)[4], const uint32_t (&rnd)[4], float& scale) {
+__device__ __forceinline__ uint32_t to_grid(const float (&x)[4], const uint32_t (&w)[4], float& scale) {
     constexpr int TOP = MANT == 3 ? 8 : 15;             // the largest value is 1.75 * 2^TOP
     constexpr int DROP = 23 - MANT;
     uint32_t b[4], amax = 0, amin = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        b[i] = __float_as_uint(x[i]) & 0x7fffffffu;
+        b[i] = SIGNED ? __float_as_uint(x[i]) & 0x7fffffffu : __float_as_uint(x[i]);
         amax = b[i] > amax ? b[i] : amax;               // as integers: a NaN is above every number
         amin = b[i] < amin ? b[i] : amin;
     }
@@ -175,31 +186,35 @@ __device__ __forceinline__ uint32_t to_grid(const float (&x)[4], const uint32_t 
     scale = __uint_as_float((uint32_t)(e + 127) << 23);
     // code = ((bits of x / scale) + random bits) >> DROP, the exponent counted from the type's; dividing by 2^e is a
     // subtraction from the exponent
-    const uint32_t shift = (uint32_t)(e + 127 - BIAS) << 23, normal = (uint32_t)(e + 128 - BIAS + 0) << 23;
-    uint32_t code[4];
+    const uint32_t shift = (uint32_t)(e + 127 - BIAS) << 23;
+    uint32_t code[4], sign = 0;
+    if (SIGNED) {                                       // the four sign bits as the codes' top bits
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x0c0c0703u);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07030c0cu);
+        sign = (lo | hi) & 0x80808080u;
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) code[i] = (b[i] + (rnd[i] << (DROP - 16)) - shift) >> DROP;
-    if (e + 128 - BIAS <= 0 || amin < normal) {
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t r = SIGNED ? (w[i] & 0xffffu) << (DROP - 16) : w[i] >> (32 - DROP) & ~((1u << (DROP - 16)) - 1u);
+        code[i] = (b[i] - shift + r) >> DROP;
+    }
+    if (e + 128 - BIAS <= 0 || amin < (uint32_t)(e + 128 - BIAS) << 23) {
         const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float t = __uint_as_float(b[i]) * inv;
+            const uint32_t r = SIGNED ? w[i] & 0xffffu : w[i] >> 16;
             if (t < __uint_as_float((uint32_t)(128 - BIAS) << 23)) {
                 const float f = t * __uint_as_float((uint32_t)(127 + BIAS - 1 + MANT + 16) << 23);
-                code[i] = ((uint32_t)(int)f + rnd[i]) >> 16;
+                code[i] = ((uint32_t)(int)f + r) >> 16;
                 if (!SIGNED && code[i] == 0u && b[i] != 0u) code[i] = 1u;       // a positive moment stays positive
+                if (SIGNED && code[i] == 0u) sign &= ~(0x80u << (8 * i));
             } else {
-                code[i] = ((__float_as_uint(t) + (rnd[i] << (DROP - 16))) >> DROP) - ((127 - BIAS) << MANT);
+                code[i] = ((__float_as_uint(t) + (r << (DROP - 16))) >> DROP) - ((127 - BIAS) << MANT);
             }
         }
     }
-    uint32_t out = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (SIGNED) code[i] |= code[i] ? __float_as_uint(x[i]) >> 24 & 0x80u : 0u;
-        out |= code[i] << (8 * i);
-    }
-    return out;
+    return (code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24) | sign;
 }
 
 // 2 x 4 elements of a chunk, a block of 256 per wave and half.  10 bytes (bf16) and some 100 instructions an element, a
@@ -249,15 +264,20 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
             const double gd = (double)gv[h][k];
             mn[k] = (float)fma((double)md[k], bm, one_b1 * gd);
             vn[k] = (float)fma(one_b2 * gd, gd, (double)vd[k] * bv);
-            if (left[h] < 4 && k >= left[h]) mn[k] = vn[k] = 0.f;       // (behind the end; a NaN scale must not get in)
-            pv[h][k] = updated(pv[h][k], mn[k], vn[k], c);
         }
+        if (left[h] < 4) {                      // behind the end (a scale that is NaN must not get in)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                mn[k] = k < left[h] ? mn[k] : 0.f;
+                vn[k] = k < left[h] ? vn[k] : 0.f;
+            }
+        }
+        update(pv[h], mn, vn, c);
         const Philox4 w = philox((uint32_t)(i >> 2), (uint32_t)((unsigned long long)i >> 34), (uint32_t)q.id, c.t,
                                  (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
-        const uint32_t wm[4] = {w.x & 0xffffu, w.y & 0xffffu, w.z & 0xffffu, w.w & 0xffffu};
-        const uint32_t wv[4] = {w.x >> 16, w.y >> 16, w.z >> 16, w.w >> 16};
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
         float msn, vsn;
-        const uint32_t mc = to_grid<3, 7, true>(mn, wm, msn), vc = to_grid<2, 15, false>(vn, wv, vsn);
+        const uint32_t mc = to_grid<3, 7, true>(mn, word, msn), vc = to_grid<2, 15, false>(vn, word, vsn);
         T* p = (T*)q.p + i;
         uint8_t *m = (uint8_t*)q.m + i, *v = (uint8_t*)q.v + i;
         if (q.vec && left[h] == 4) {
@@ -282,7 +302,7 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
 // One chunk per workgroup.  (As many workgroups as fit, each walking every so many chunks, take 20 % longer: they do not
 // end together.)
 template <int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(const AdamWArgs a) {
+__global__ __launch_bounds__(256, BITS == 8 ? 6 : 4) void adamw_kernel(const AdamWArgs a) {
     for (long long k = blockIdx.x; k < a.n_chunks; k += gridDim.x) {
         const sca_adamw_chunk ch = a.chunks[k];
         const sca_adamw_tensor q = a.tensors[ch.tensor];

@@ -697,6 +697,37 @@ def test_adamw_under_graph_capture(ops, bits):
             b.step()
 
 
+def test_adamw_is_a_torch_optimizer(ops):
+    """Step hooks run once per step, schedulers change the rate, a closure is called and its value returned, parameters may
+    join later."""
+    p = tensors([(20,), (30,)], torch.float32, 4)
+    q = [x.clone() for x in p]
+    opt = ops.AdamW(p[:1], lr=0.1, weight_decay=0.0)
+    calls = []
+    opt.step()
+    opt.register_step_pre_hook(lambda o, a, k: calls.append("pre"))
+    handle = opt.register_step_post_hook(lambda o, a, k: calls.append("post"))
+    assert opt.step(lambda: 3.5) == 3.5 and calls == ["pre", "post"]
+    handle.remove()
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    opt.add_param_group(dict(params=p[1:], lr=0.2))
+    opt.step()
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 0.05
+    opt.step()
+    ref = torch.optim.AdamW([x.double() for x in q[:1]], lr=0.1, weight_decay=0.0)
+    y = ref.param_groups[0]["params"][0]
+    y.grad = p[0].grad.double()
+    for lr in (0.1, 0.1, 0.1, 0.05):
+        ref.param_groups[0]["lr"] = lr
+        ref.step()
+    within(p[0], y, 4 * 20 * U * (y.abs() + 0.1), "p")
+    assert [v["step"] for v in opt.state_dict()["state"].values()] == [4, 2]
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any("AdamW.step" in e.key for e in prof.key_averages())
+
+
 def test_adamw_offsets_past_32_bits(ops):
     n = (1 << 31) + 1111
     x = torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16)
