@@ -222,6 +222,8 @@ class CVAEEngine:
             self.p[k].copy_(named_params[k].detach().to(torch.float32))
         self.trainable = {k: True for k in self.names}
         self.adam_t = 0
+        self.optimizer = "adam"         # set_optimizer
+        self._adamw_tables = {}
 
         # ---- layer table -----------------------------------------------------------------------------------
         H, G, Z = self.H, self.G, self.Z
@@ -1769,12 +1771,43 @@ class CVAEEngine:
                 open_wd = wd
         return [(s, e, wd) for s, e, wd in merged]
 
+    def set_optimizer(self, name: str):
+        """"adam": torch.optim.Adam with the decay folded into the gradient, as the reference trains; "adamw":
+        torch.optim.AdamW (decay decoupled from the gradient).  Both read the same moments, hyper[] and decays."""
+        if name not in ("adam", "adamw"):
+            raise ValueError(f"optimizer must be 'adam' or 'adamw', not {name!r}")
+        self.optimizer = name
+
+    def _adamw_table(self, ranges):
+        """Device table of sca_adamw_step over ranges of the flat buffers (built once per set of ranges; the warm-up pass
+        of a recorded or captured step builds it)."""
+        tab = self._adamw_tables.get(ranges)
+        if tab is None:
+            raw = self.lib._lib
+            chunk = raw.sca_adamw_chunk_elements()
+            rows = [_lib.AdamWTensor(self.flat_p[s:].data_ptr(), self.flat_g[s:].data_ptr(), self.flat_m[s:].data_ptr(),
+                                     self.flat_v[s:].data_ptr(), None, None, e - s, None, wd, 0, int(s % 4 == 0), j)
+                    for j, (s, e, wd) in enumerate(ranges)]
+            chunks = np.array([(j, k) for j, r in enumerate(rows) for k in range(-(-r.n // chunk))], dtype=np.int32)
+            size = raw.sca_adamw_scratch_bytes(len(rows))
+            host = bytes(size) + bytes((_lib.AdamWTensor * len(rows))(*rows)) + chunks.tobytes()
+            dev = torch.from_numpy(np.frombuffer(host, dtype=np.uint8).copy()).to(self.device)
+            at = dev.data_ptr()
+            tab = self._adamw_tables[ranges] = (dev, at + size, len(rows), at + len(host) - chunks.nbytes, len(chunks), at)
+        return tab[1:]
+
     def adam_step(self, weight_decay=0.04, wd_overrides: Optional[Dict[str, float]] = None, stream=None):
-        """One torch.optim.Adam-equivalent update of every trainable tensor; hyper[] must hold lr / bias corrections
-        for step t = self.adam_t + 1 (call begin_step first).  wd_overrides: per-tensor weight decay (scPoli keeps its
-        embeddings in a weight_decay=0 parameter group, trainers/scpoli/trainer.py:297-305)."""
+        """One torch.optim.Adam-equivalent update of every trainable tensor (torch.optim.AdamW after
+        set_optimizer("adamw")); hyper[] must hold lr / bias corrections for step t = self.adam_t + 1 (call begin_step
+        first).  wd_overrides: per-tensor weight decay (scPoli keeps its embeddings in a weight_decay=0 parameter group,
+        trainers/scpoli/trainer.py:297-305)."""
         L = self.lib
         st = stream if stream is not None else torch.cuda.current_stream(self.device).cuda_stream
+        if self.optimizer == "adamw":
+            entries, n, chunks, n_chunks, scratch = self._adamw_table(tuple(self.trainable_ranges(weight_decay, wd_overrides)))
+            _lib.check(L.sca_adamw_step(entries, n, chunks, n_chunks, 32, self.hyper.data_ptr(), 0.0, 0.9, 0.999, 0.0, 0,
+                                        scratch, st), "adamw")
+            return
         for s, e, wd in self.trainable_ranges(weight_decay, wd_overrides):
             _lib.check(L.sca_adam_step(self.flat_p[s:].data_ptr(), self.flat_g[s:].data_ptr(),
                                        self.flat_m[s:].data_ptr(), self.flat_v[s:].data_ptr(), e - s,
@@ -1977,7 +2010,7 @@ class CVAEEngine:
                     tuple(sorted(k for k, v in self.trainable.items() if v)), self.use_mmd, self.mmd_on,
                     self.boundary, self.beta, torch.cuda.current_stream(self.device).cuda_stream,
                     self._dp_n_global if dp_exact else None, self.hsic_beta, self.dr_rate, self.seed, self.freeze,
-                    self._ws_gen, self._pf_flags)
+                    self.optimizer, self._ws_gen, self._pf_flags)
         self._ensure(B)
         # (launch plans only: captured into a HIP graph the trailing gather costs more than the head gather it
         #  replaces - 0.350 -> 0.360 ms at 4096 cells, 0.239 -> 0.245 ms at 1024)
@@ -2156,8 +2189,29 @@ class CVAEEngine:
                    "begin_step")
 
     # ------------------------------------------------------------------------------------------ inference
-    def encode(self, row_ids, cond, B, mean=True, x_dense=None, eps=None, covs=None):
-        """Eval-mode encoder pass: returns (z or mean [B,Z], mean, var) device tensors (views of the workspace)."""
+    def quantize_first_layer(self):
+        """(wq, scale) of the first encoder layer's weight for encode(int8=...): 8-bit integers with one scale per output."""
+        from . import ops
+        return ops.quantize_int8(self.p[self.enc[0].w])
+
+    def _first_product(self, a, B, st, int8, max_split=None):
+        """x W0^T of the first encoder layer as (ptr, slabs, stride): fp32, or in 8-bit integers with one scale per cell
+        and per output (`int8` = quantize_first_layer())."""
+        ly = self.enc[0]
+        if int8 is None:
+            return self._gemm(0, 0, a, ly.n_in, self.p[ly.w].data_ptr(), ly.n_in, B, ly.n_out, ly.n_in, st,
+                              max_split=max_split)
+        wq, scale = int8
+        raw, slab = self.lib._lib, self.ws["slab"]
+        size = raw.sca_linear_i8_workspace_bytes(B, ly.n_in)
+        scratch = torch.empty(size, dtype=torch.int8, device=self.device) if size else None
+        _lib.check(raw.sca_linear_i8(a, ly.n_in, 0, wq.data_ptr(), wq.stride(0), scale.data_ptr(), None, 0, B, ly.n_out,
+                                     ly.n_in, slab.data_ptr(), 0, ly.n_out, _lib.ptr(scratch), st), "linear_i8")
+        return slab.data_ptr(), 1, B * ly.n_out
+
+    def encode(self, row_ids, cond, B, mean=True, x_dense=None, eps=None, covs=None, int8=None):
+        """Eval-mode encoder pass: returns (z or mean [B,Z], mean, var) device tensors (views of the workspace).
+        `int8` (quantize_first_layer()): the first layer's product, nearly all of the pass, in 8-bit integers."""
         L, P = self.lib, self.p
         self._pf = None         # ws["x"] is about to be overwritten
         self._ensure(B)
@@ -2180,8 +2234,7 @@ class CVAEEngine:
             # first-layer GEMM, then ONE launch for its epilogue, the remaining encoder layers, the heads and the latent
             # block (sca_mid_fwd with n_dec = 0) instead of a GEMM + epilogue pair per layer
             ly = self.enc[0]
-            pre0 = self._gemm(0, 0, a, ly.n_in, P[ly.w].data_ptr(), ly.n_in, B, ly.n_out, ly.n_in, st,
-                              max_split=self._mid_max_split)
+            pre0 = self._first_product(a, B, st, int8, self._mid_max_split)
             self.step_ctr += 1          # fresh noise for every sampled pass
             _lib.check(L.sca_mid_fwd(self._mid_args(B, cond_p, 0.0, eps, {}, pre0=pre0, sample=0 if mean else 1,
                                                     encoder_only=True), st), "mid_fwd[encode]")
@@ -2194,7 +2247,10 @@ class CVAEEngine:
         else:
             cw, cwp, cvec_p, cE = C, cond_p, None, 0
         for ly in self.enc:
-            sp, S, stride = self._gemm(0, 0, a, ly.n_in, P[ly.w].data_ptr(), ly.n_in, B, ly.n_out, ly.n_in, st)
+            if ly is self.enc[0]:
+                sp, S, stride = self._first_product(a, B, st, int8)
+            else:
+                sp, S, stride = self._gemm(0, 0, a, ly.n_in, P[ly.w].data_ptr(), ly.n_in, B, ly.n_out, ly.n_in, st)
             a = self._layer_block_fwd(ly, sp, S, stride, B, (cw, cwp, cvec_p, cE), 0.0, None, False, None, st)
         Hl = self.H[-1]
         sp, S, stride = self._gemm(0, 0, a, Hl, self.heads_w.data_ptr(), Hl, B, 2 * Z, Hl, st)

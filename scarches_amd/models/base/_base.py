@@ -162,9 +162,11 @@ class CVAELatentsMixin:
                      torch.from_numpy(csr.data.astype(np.float32)).to(eng.device))
         return csr.shape[0]
 
-    def get_latent(self, x=None, c=None, mean: bool = False, mean_var: bool = False):
+    def get_latent(self, x=None, c=None, mean: bool = False, mean_var: bool = False, int8: bool = False):
         """Latent representation of `x` (default: self.adata.X) given condition labels `c`.
-        mean=True: encoder means; mean_var=True: (means, variances); otherwise a sample z."""
+        mean=True: encoder means; mean_var=True: (means, variances); otherwise a sample z.
+        int8=True: the first layer's product in 8-bit integers with one scale per cell and per output - an approximation
+        for mapping large data sets (each factor is rounded to 1 / 127 of its row's largest value)."""
         if x is None and c is None:
             x = self.adata.X
             if self.conditions_ is not None:
@@ -174,11 +176,13 @@ class CVAELatentsMixin:
         if c is not None:
             labels = torch.from_numpy(self._encode_labels(c)).to(eng.device)
         n = self._upload(x, eng)
+        weight = eng.quantize_first_layer() if int8 else None
         outs = []
         for lo in range(0, n, self._LATENT_BLOCK):
             hi = min(n, lo + self._LATENT_BLOCK)
             rows = torch.arange(lo, hi, device=eng.device, dtype=torch.int64)
-            z, mu, var = eng.encode(rows, None if labels is None else labels[lo:hi].contiguous(), hi - lo, mean=False)
+            z, mu, var = eng.encode(rows, None if labels is None else labels[lo:hi].contiguous(), hi - lo, mean=False,
+                                    int8=weight)
             if mean:
                 outs.append((mu.cpu(),))
             elif mean_var:

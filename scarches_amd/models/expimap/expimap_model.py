@@ -90,9 +90,9 @@ class EXPIMAP(BaseMixin, SurgeryMixin, CVAELatentsMixin):
         return self.model.decoder.nonzero_terms()
 
     def get_latent(self, x: Optional[np.ndarray] = None, c: Optional[np.ndarray] = None, only_active: bool = False,
-                   mean: bool = False, mean_var: bool = False):
+                   mean: bool = False, mean_var: bool = False, int8: bool = False):
         """As CVAELatentsMixin.get_latent; only_active keeps the columns of active terms."""
-        result = super().get_latent(x, c, mean, mean_var)
+        result = super().get_latent(x, c, mean, mean_var, int8)
         if not only_active:
             return result
         idx = self.nonzero_terms()

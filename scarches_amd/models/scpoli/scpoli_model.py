@@ -159,7 +159,7 @@ class scPoli(BaseMixin):
             cols.append(lab)
         return np.stack(cols, 1)
 
-    def _latent_blocks(self, x, covs, mean):
+    def _latent_blocks(self, x, covs, mean, int8=False):
         eng = self.model.engine()
         csr = x.tocsr().astype(np.float32) if sp.issparse(x) else sp.csr_matrix(np.asarray(x, dtype=np.float32))
         if not csr.has_canonical_format:
@@ -171,16 +171,18 @@ class scPoli(BaseMixin):
         covs = torch.from_numpy(covs).to(eng.device)
         n = csr.shape[0]
         out = torch.empty(n, eng.Zt, device=eng.device)
+        weight = eng.quantize_first_layer() if int8 else None
         for lo in range(0, n, _BLOCK):
             hi = min(n, lo + _BLOCK)
             rows = torch.arange(lo, hi, device=eng.device, dtype=torch.int64)
-            z, mu, _ = eng.encode(rows, None, hi - lo, mean=False, covs=covs[lo:hi].contiguous())
+            z, mu, _ = eng.encode(rows, None, hi - lo, mean=False, covs=covs[lo:hi].contiguous(), int8=weight)
             out[lo:hi].copy_(mu if mean else z)
         return out
 
-    def get_latent(self, adata, mean: bool = False):
-        """Latent representation (sample, or mean with mean=True) of `adata` as a numpy array [n_obs, latent_dim]."""
-        return self._latent_blocks(adata.X, self._encode_covariates(adata.obs), mean).cpu().numpy()
+    def get_latent(self, adata, mean: bool = False, int8: bool = False):
+        """Latent representation (sample, or mean with mean=True) of `adata` as a numpy array [n_obs, latent_dim].
+        int8=True: the first layer's product in 8-bit integers (an approximation for mapping large data sets)."""
+        return self._latent_blocks(adata.X, self._encode_covariates(adata.obs), mean, int8).cpu().numpy()
 
     def get_conditional_embeddings(self):
         """Learnt condition embeddings: a CellData per condition key (obs index = condition names); a single object

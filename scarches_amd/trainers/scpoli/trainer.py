@@ -55,6 +55,8 @@ class scPoliTrainer(Trainer):
         self.use_stratified_sampling = kwargs.pop("use_stratified_sampling", False)
         self.weight_decay = kwargs.pop("weight_decay", 0.04)
         self.clip_value = kwargs.pop("clip_value", 0.0)
+        # of the network's parameters; unlabeled prototypes keep Adam
+        self.optimizer_name = kwargs.pop("optimizer", "adam")
         self.n_workers = kwargs.pop("n_workers", 0)
         self.seed = kwargs.pop("seed", 2020)
         self.monitor = kwargs.pop("monitor", True)

@@ -60,6 +60,8 @@ class Trainer:
         self.use_stratified_sampling = kwargs.pop("use_stratified_sampling", True)
         self.weight_decay = kwargs.pop("weight_decay", 0.04)
         self.clip_value = kwargs.pop("clip_value", 0.0)
+        # "adam" (the reference's: decay folded into the gradient) or "adamw" (decoupled decay, CVAEEngine.set_optimizer)
+        self.optimizer_name = kwargs.pop("optimizer", "adam")
         self.n_workers = kwargs.pop("n_workers", 0)          # accepted for compatibility; there are no host workers
         self.seed = kwargs.pop("seed", 2020)
         self.monitor = kwargs.pop("monitor", True)
@@ -204,6 +206,7 @@ class Trainer:
         """The reference builds a new torch.optim.Adam in every train() (trainer.py:221-223): moments and the
         bias-correction step restart from zero; the engine's Philox seed follows this trainer's seed."""
         eng = self.engine
+        eng.set_optimizer(self.optimizer_name)
         eng.flat_m.zero_()
         eng.flat_v.zero_()
         eng.adam_t = 0
