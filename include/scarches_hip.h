@@ -351,7 +351,7 @@ int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, long long l
 /* ---- AdamW over a list of tensors ----------------------------------------------------------------------------------
  * m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  * p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * for every tensor of a table in one step of two launches, however many there are (torch.optim.AdamW; sca_adam_step is the coupled form on one range).
+ * for every tensor of a table in one or two launches, however many there are (torch.optim.AdamW; sca_adam_step is the coupled form on one range).
  * `tensors` and `chunks` lie in DEVICE memory: one sca_adamw_tensor per tensor, and for tensor j the entries {j, 0}, {j, 1},
  * ... of ceil(n / sca_adamw_chunk_elements()) chunks.  p and g: dtype 0 fp32, 1 bf16, 2 fp16 (computed in fp32, rounded
  * once).  vec = 1 promises that p, g and - with 32-bit states - m, v are aligned to 4 of their elements, and with 8-bit
@@ -360,10 +360,11 @@ int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, long long l
  * value * scale with one fp32 power of two per sca_adamw_block_elements() consecutive elements in m_scale / v_scale;
  * rounding is stochastic: the 16 low (m) / high (v) bits of word i & 3 of Philox4x32-10(counter (i >> 2, id, t), key seed)
  * decide for element i (common.h's generator).  A block with a value that is not finite keeps scale NaN.
- * Step number: hyper != NULL (32-bit states only) reads lr, the bias corrections, eps and the clip value from the block that
- * sca_begin_step fills; hyper = NULL uses lr / eps as given, advances every *step of the table by 1 and takes the result as
- * t.  scratch: sca_adamw_scratch_bytes(n_tensors) bytes, 16-byte aligned, any contents on entry; it, the steps and the
- * tensors belong to one step at a time.  No tensor may appear twice in a table. */
+ * Step number: hyper != NULL (32-bit states only, t = 0) reads lr, the bias corrections, eps and the clip value from the
+ * block that sca_begin_step fills.  hyper = NULL uses lr / eps as given and, t > 0: t for all tensors, every *step of the
+ * table becomes t (one launch); t = 0: every *step advances by 1 and counts for its tensor (a launch more; what a captured
+ * step takes, since its replays count on).  scratch (t = 0): sca_adamw_scratch_bytes(n_tensors) bytes, 16-byte aligned, any
+ * contents on entry; it, the steps and the tensors belong to one step at a time.  No tensor may appear twice in a table. */
 typedef struct {
     void* p; const void* g; void* m; void* v;
     float* m_scale; float* v_scale;
@@ -379,8 +380,8 @@ int sca_adamw_chunk_elements(void);
 int sca_adamw_block_elements(void);
 long long sca_adamw_scratch_bytes(int n_tensors);
 int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_adamw_chunk* chunks, int n_chunks,
-                   int state_bits, const float* hyper, float lr, double beta1, double beta2, float eps, uint64_t seed,
-                   void* scratch, void* stream);
+                   int state_bits, const float* hyper, long long t, float lr, double beta1, double beta2, float eps,
+                   uint64_t seed, void* scratch, void* stream);
 
 /* ---- product in 8-bit integers -------------------------------------------------------------------------------------
  * sca_quant_rows_i8: scale[r] = max_k |x_rk| / 127, q_rk = round(x_rk / scale[r]) (ties to even, the exact quotient), and

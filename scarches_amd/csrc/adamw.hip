@@ -4,9 +4,10 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)        (decoupled decay)
 //
 // A step walks a table of tensors that lies in device memory (one entry per tensor, one per chunk of 2048 elements), so
-// the number of tensors costs no launches.  The step numbers live in device memory as well: a small launch in front
-// advances them and derives every tensor's coefficients (in 64 bits, once, instead of in every workgroup), so a captured
-// step counts on when it is replayed.
+// the number of tensors costs no launches.  The step numbers live in device memory as well, so that a captured step counts
+// on when it is replayed: a small launch in front advances them and derives every tensor's coefficients (in 64 bits, once,
+// instead of in every workgroup).  A caller that knows the step number gives it and does without that launch (3 us of 15
+// for a small network); the numbers in memory are kept up all the same.
 //
 // 8-bit states: every 256 elements of a tensor share a power-of-two scale per moment, with m / scale held as e4m3 and
 // v / scale as e5m2 floats (v spans twice the exponents of m).  Rounding to that grid is stochastic: at b2 = 0.999 a step
@@ -25,16 +26,29 @@ constexpr int CHUNK = 2048;         // elements per table chunk: 8 per thread, l
 constexpr int QBLOCK = 256;         // elements per 8-bit scale: one wave, four consecutive elements per lane
 
 struct Coef {                       // what a step needs to know of a tensor
-    float decay, step_size, inv_bc2, eps, clip;
+    float lr, step_size, inv_bc2, eps, clip;
     uint32_t t;
     uint32_t pad[2];
 };
 static_assert(sizeof(Coef) == 32, "sca_adamw_scratch_bytes");
 
+// Of step t: lr / (1 - beta1^t) and 1 / sqrt(1 - beta2^t), without the cancellation.
+__host__ __device__ inline Coef coef_of(int64_t t, float lr, float eps, double log_beta1, double log_beta2) {
+    Coef c = {};
+    c.lr = lr;
+    c.step_size = lr / (float)-expm1((double)t * log_beta1);
+    c.inv_bc2 = 1.0f / (float)sqrt(-expm1((double)t * log_beta2));
+    c.eps = eps;
+    c.t = (uint32_t)t;
+    return c;
+}
+
 struct AdamWArgs {
     const sca_adamw_tensor* tensors;
     const sca_adamw_chunk* chunks;
-    Coef* coef;                     // [n_tensors]
+    Coef* coef;                     // [n_tensors], or null: `given` for all
+    Coef given;
+    int64_t t;                      // with `given`: what the tensors' steps become
     int n_chunks, n_tensors;
     const float* hyper;             // sca_begin_step's block, or null: the scalars below and the tensors' own steps
     float lr, eps;
@@ -48,27 +62,25 @@ __global__ __launch_bounds__(256) void adamw_begin_kernel(const AdamWArgs a) {
     if (j >= a.n_tensors) return;
     const sca_adamw_tensor q = a.tensors[j];
     Coef c = {};
-    float lr = a.lr, bc1, bc2s;
     if (a.hyper) {
-        lr = a.hyper[1]; bc1 = a.hyper[2]; bc2s = a.hyper[3]; c.eps = a.hyper[4]; c.clip = a.hyper[5];
+        c.lr = a.hyper[1];
+        c.step_size = a.hyper[1] / a.hyper[2];
+        c.inv_bc2 = 1.0f / a.hyper[3];
+        c.eps = a.hyper[4];
+        c.clip = a.hyper[5];
     } else {
         const int64_t t = *q.step + 1;
         *q.step = t;
-        bc1 = (float)-expm1((double)t * a.log_beta1);           // 1 - beta^t without the cancellation
-        bc2s = (float)sqrt(-expm1((double)t * a.log_beta2));
-        c.eps = a.eps;
-        c.t = (uint32_t)t;
+        c = coef_of(t, a.lr, a.eps, a.log_beta1, a.log_beta2);
     }
-    c.decay = 1.0f - lr * q.weight_decay;
-    c.step_size = lr / bc1;
-    c.inv_bc2 = 1.0f / bc2s;
     a.coef[j] = c;
 }
 
 // p of four elements.  denom = sqrt(v) / sqrt(1 - b2^t) + eps; v_sqrt_f32 and v_rcp_f32 are good to one unit in the last
 // place where their arguments are ordinary numbers, the exact sequences (some 25 instructions) are for what is near the
 // denormal ones.
-__device__ __forceinline__ void update(float (&p)[4], const float (&m)[4], const float (&v)[4], const Coef& c) {
+__device__ __forceinline__ void update(float (&p)[4], const float (&m)[4], const float (&v)[4], const Coef& c,
+                                       float decay) {
     float denom[4], q[4], lo = 1e30f, hi = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -82,7 +94,7 @@ __device__ __forceinline__ void update(float (&p)[4], const float (&m)[4], const
         for (int k = 0; k < 4; ++k) q[k] = m[k] / fmaf(sqrtf(v[k]), c.inv_bc2, c.eps);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = fmaf(-c.step_size, q[k], p[k] * c.decay);
+    for (int k = 0; k < 4; ++k) p[k] = fmaf(-c.step_size, q[k], p[k] * decay);
 }
 
 // ---- 32-bit states ------------------------------------------------------------------------------------------------------
@@ -114,7 +126,7 @@ __device__ __forceinline__ void chunk32(const sca_adamw_tensor& q, long long i0,
             mv[h][k] = fmaf(a.b1, mv[h][k], a.one_minus_b1 * gk);
             vv[h][k] = fmaf(a.b2, vv[h][k], a.one_minus_b2 * gk * gk);
         }
-        update(pv[h], mv[h], vv[h], c);
+        update(pv[h], mv[h], vv[h], c, 1.0f - c.lr * q.weight_decay);
         T* p = (T*)q.p + i;
         float *m = (float*)q.m + i, *v = (float*)q.v + i;
         if (q.vec && left[h] == 4) {
@@ -272,7 +284,7 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
                 vn[k] = k < left[h] ? vn[k] : 0.f;
             }
         }
-        update(pv[h], mn, vn, c);
+        update(pv[h], mn, vn, c, 1.0f - c.lr * q.weight_decay);
         const Philox4 w = philox((uint32_t)(i >> 2), (uint32_t)((unsigned long long)i >> 34), (uint32_t)q.id, c.t,
                                  (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
         const uint32_t word[4] = {w.x, w.y, w.z, w.w};
@@ -303,10 +315,12 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
 // end together.)
 template <int BITS>
 __global__ __launch_bounds__(256, BITS == 8 ? 6 : 4) void adamw_kernel(const AdamWArgs a) {
+    if (!a.coef && blockIdx.x == 0)             // (nothing in this launch reads the steps)
+        for (int j = threadIdx.x; j < a.n_tensors; j += 256) *a.tensors[j].step = a.t;
     for (long long k = blockIdx.x; k < a.n_chunks; k += gridDim.x) {
         const sca_adamw_chunk ch = a.chunks[k];
         const sca_adamw_tensor q = a.tensors[ch.tensor];
-        const Coef c = a.coef[ch.tensor];
+        const Coef c = a.coef ? a.coef[ch.tensor] : a.given;
         const long long i = (long long)ch.index * CHUNK + 4 * threadIdx.x;
         if (BITS == 32) {
             if (q.dtype == SCA_F32) chunk32<float>(q, i, c, a);
@@ -327,18 +341,21 @@ extern "C" int sca_adamw_block_elements(void) { return QBLOCK; }
 extern "C" long long sca_adamw_scratch_bytes(int n_tensors) { return n_tensors < 0 ? -1 : (long long)n_tensors * sizeof(Coef); }
 
 extern "C" int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_adamw_chunk* chunks,
-                              int n_chunks, int state_bits, const float* hyper, float lr, double beta1, double beta2,
-                              float eps, uint64_t seed, void* scratch, void* stream) {
-    if (n_tensors < 0 || n_chunks < 0 || (state_bits != 32 && state_bits != 8)) return -1;
+                              int n_chunks, int state_bits, const float* hyper, long long t, float lr, double beta1,
+                              double beta2, float eps, uint64_t seed, void* scratch, void* stream) {
+    if (n_tensors < 0 || n_chunks < 0 || (state_bits != 32 && state_bits != 8) || t < 0) return -1;
     if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return -1;
-    if (hyper ? state_bits != 32 : !(eps >= 0.f)) return -1;
+    if (hyper ? state_bits != 32 || t != 0 : !(eps >= 0.f)) return -1;
     if (n_tensors == 0) return 0;
-    if (!tensors || !scratch || ((uintptr_t)scratch & 15) || (n_chunks > 0 && !chunks)) return -1;
+    if (!tensors || (n_chunks > 0 && !chunks)) return -1;
+    if (t == 0 && (!scratch || ((uintptr_t)scratch & 15))) return -1;
     hipStream_t st = (hipStream_t)stream;
-    const AdamWArgs a{tensors, chunks, (Coef*)scratch, n_chunks, n_tensors, hyper, lr, eps, beta1, beta2, log(beta1),
-                      log(beta2), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), seed};
-    hipLaunchKernelGGL(adamw_begin_kernel, dim3((n_tensors + 255) / 256), dim3(256), 0, st, a);
-    const int grid = n_chunks < (1 << 23) ? n_chunks : 1 << 23;         // fewer than 2^32 threads
+    AdamWArgs a{tensors, chunks, t ? nullptr : (Coef*)scratch, Coef{}, t, n_chunks, n_tensors, hyper, lr, eps, beta1, beta2,
+                log(beta1), log(beta2), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), seed};
+    if (t) a.given = coef_of(t, lr, eps, a.log_beta1, a.log_beta2);
+    else hipLaunchKernelGGL(adamw_begin_kernel, dim3((n_tensors + 255) / 256), dim3(256), 0, st, a);
+    int grid = n_chunks < (1 << 23) ? n_chunks : 1 << 23;               // fewer than 2^32 threads
+    if (t && grid == 0) grid = 1;                                       // (the steps)
     if (grid > 0 && state_bits == 32) hipLaunchKernelGGL((adamw_kernel<32>), dim3(grid), dim3(256), 0, st, a);
     else if (grid > 0) hipLaunchKernelGGL((adamw_kernel<8>), dim3(grid), dim3(256), 0, st, a);
     SCA_CHECK_LAUNCH();

@@ -1805,8 +1805,8 @@ class CVAEEngine:
         st = stream if stream is not None else torch.cuda.current_stream(self.device).cuda_stream
         if self.optimizer == "adamw":
             entries, n, chunks, n_chunks, scratch = self._adamw_table(tuple(self.trainable_ranges(weight_decay, wd_overrides)))
-            _lib.check(L.sca_adamw_step(entries, n, chunks, n_chunks, 32, self.hyper.data_ptr(), 0.0, 0.9, 0.999, 0.0, 0,
-                                        scratch, st), "adamw")
+            _lib.check(L.sca_adamw_step(entries, n, chunks, n_chunks, 32, self.hyper.data_ptr(), 0, 0.0, 0.9, 0.999, 0.0,
+                                        0, scratch, st), "adamw")
             return
         for s, e, wd in self.trainable_ranges(weight_decay, wd_overrides):
             _lib.check(L.sca_adam_step(self.flat_p[s:].data_ptr(), self.flat_g[s:].data_ptr(),

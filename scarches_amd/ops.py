@@ -324,6 +324,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 8 or 32, not {state_bits}")
         self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFFFFFFFFFF
         self._steps = {}            # group number -> int64 [parameters] on the device: their steps
+        self._host_steps = {}       # group number -> the step of all its parameters, None where only the device knows
         self._plans = {}            # group number -> the table of the last step()
         self._captured = []         # tables (and what they point to) that captured graphs read
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -366,6 +367,8 @@ class AdamW(torch.optim.Optimizer):
         """Set the number of steps that every parameter has behind it (a run taken up from states of another program)."""
         for gi in range(len(self.param_groups)):
             self._group_steps(gi).fill_(int(step))
+            if self._host_steps.get(gi, 0) is not None:
+                self._host_steps[gi] = int(step)
 
     def state_dict(self):
         """torch's layout; every parameter's state has `step` as a whole number (read from the device)."""
@@ -396,6 +399,8 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p] = {k: st[k].to(p.device, torch.float32 if self.state_bits == 32 else st[k].dtype,
                                                  copy=True) for k in keys}
             self._group_steps(gi).copy_(torch.tensor(steps))
+            if self._host_steps.get(gi, 0) is not None:
+                self._host_steps[gi] = steps[0] if len(set(steps)) == 1 else None
 
     # ------------------------------------------------------------------------------------------ step
     def _table(self, gi, group, key):
@@ -448,8 +453,8 @@ class AdamW(torch.optim.Optimizer):
         host = torch.from_numpy(np.frombuffer(bytes(size) + entries + chunks.tobytes(), dtype=np.uint8).copy()).pin_memory()
         table = host.to(dev, non_blocking=True)
         at = table.data_ptr() + size
-        return dict(key=key, table=table, streams={_raw_stream(dev.index)}, entries=at, n=len(rows), chunks=at + len(entries), n_chunks=len(chunks),
-                    steps=steps, scratch=table.data_ptr(), index=dev.index)
+        return dict(key=key, table=table, streams={_raw_stream(dev.index)}, entries=at, n=len(rows), chunks=at + len(entries),
+                    n_chunks=len(chunks), steps=steps, scratch=table.data_ptr(), index=dev.index)
 
     def _step(self, closure=None):
         loss = None
@@ -463,6 +468,7 @@ class AdamW(torch.optim.Optimizer):
             for p in group["params"]:
                 g = p.grad
                 if g is None:
+                    self._host_steps[gi] = None
                     continue
                 st = self.state[p]
                 if not st:
@@ -481,11 +487,16 @@ class AdamW(torch.optim.Optimizer):
                 plan["streams"].add(stream)
                 if not torch.cuda.is_current_stream_capturing():
                     plan["table"].record_stream(torch.cuda.current_stream(plan["table"].device))
+            # As long as all parameters have taken every step and no graph takes steps that nobody here sees, the step number
+            # is given; else the device counts.
+            t = self._host_steps.get(gi, 0)
             if torch.cuda.is_current_stream_capturing():    # replays read the table and what it points to
                 self._captured.append((plan, [(p, p.grad, dict(self.state[p])) for p in group["params"]]))
+                t = None
+            t = self._host_steps[gi] = None if t is None else t + 1
             b1, b2 = group["betas"]
             _call(plan["index"], "sca_adamw_step", plan["entries"], plan["n"], plan["chunks"], plan["n_chunks"],
-                  self.state_bits, None, group["lr"], b1, b2, group["eps"], self.seed, plan["scratch"])
+                  self.state_bits, None, t or 0, group["lr"], b1, b2, group["eps"], self.seed, plan["scratch"])
         return loss
 
     # torch wraps step() to run its hooks and to be seen by the profiler, which takes 6 us: here only where one is wanted

@@ -113,7 +113,8 @@ def test_entry_points_check_their_arguments():
         assert lib.sca_linear_i8(*ok[:i], bad, *ok[i + 1:]) == -1, i
     assert lib.sca_linear_i8_workspace_bytes(40, 8) == 40 * 132 and lib.sca_linear_i8_workspace_bytes(1, 8) == 0
     assert lib.sca_linear_i8_workspace_bytes(-1, 8) == -1 and lib.sca_linear_i8_workspace_bytes(1, 1 << 17) == -1
-    ok = (a, 1, a, 1, 32, None, 1e-3, 0.9, 0.999, 1e-8, 0, a, None)
-    for i, bad in ((0, None), (1, -1), (2, None), (3, -1), (4, 16), (7, 1.0), (8, -0.1), (9, -1.0), (11, None), (11, a + 8)):
+    ok = (a, 1, a, 1, 32, None, 0, 1e-3, 0.9, 0.999, 1e-8, 0, a, None)
+    for i, bad in ((0, None), (1, -1), (2, None), (3, -1), (4, 16), (6, -1), (8, 1.0), (9, -0.1), (10, -1.0), (12, None), (12, a + 8)):
         assert lib.sca_adamw_step(*ok[:i], bad, *ok[i + 1:]) == -1, i
-    assert lib.sca_adamw_step(a, 1, a, 1, 8, a, 1e-3, 0.9, 0.999, 1e-8, 0, a, None) == -1      # hyper: 32 bits only
+    assert lib.sca_adamw_step(a, 1, a, 1, 8, a, 0, 1e-3, 0.9, 0.999, 1e-8, 0, a, None) == -1       # hyper: 32 bits only
+    assert lib.sca_adamw_step(a, 1, a, 1, 32, a, 3, 1e-3, 0.9, 0.999, 1e-8, 0, a, None) == -1      # and no step number
