@@ -337,9 +337,9 @@ int sca_bn_bwd(const float* dh, int S, long long slab_stride, const float* extra
  * dtype of x, y, dy, dx: 0 fp32, 1 bf16, 2 fp16; wtype of w, b, dw, db: 0 or dtype.  Rows of pitch ld* elements (>= n for
  * outputs; any pitch from 0 - one row read again and again - for inputs), any alignment.  w / b may be NULL (1 / 0).
  * stats [2][rows] = (mean, rstd), fp32; may be NULL in the forward pass.  Sums and statistics are held in fp32, each
- * result is rounded once.  sca_layernorm_bwd: dx, dw, db may each be NULL; ws: scratch of
- * sca_layernorm_bwd_workspace_floats(rows, n) floats, only for dw / db (any contents on entry; a workspace must not be
- * shared by calls that may overlap).  Sums over rows are taken in a fixed order: the same call gives the same bits.
+ * result is rounded once.  Outputs overlap no input.  sca_layernorm_bwd: dx, dw, db may
+ * each be NULL; ws: scratch of sca_layernorm_bwd_workspace_floats(rows, n) floats (any contents on entry; not to be shared
+ * by calls that may overlap), which may be NULL where neither dw nor db is asked for and n <= 16384.  Sums over rows are taken in a fixed order: the same call gives the same bits.
  * rows = 0: nothing is read, dw and db become 0.  -1 for an argument outside these ranges. */
 int sca_layernorm_fwd(const void* x, long long ldx, int dtype, long long rows, int n, const void* w, const void* b,
                       int wtype, float eps, void* y, long long ldy, float* stats, void* stream);
@@ -351,7 +351,8 @@ int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, long long l
 /* ---- AdamW over a list of tensors ----------------------------------------------------------------------------------
  * m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  * p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * for every tensor of a table in one or two launches, however many there are (torch.optim.AdamW; sca_adam_step is the coupled form on one range).
+ * for every tensor of a table in one or two launches, however many there are (torch.optim.AdamW; sca_adam_step is the
+ * coupled form on one range).
  * `tensors` and `chunks` lie in DEVICE memory: one sca_adamw_tensor per tensor, and for tensor j the entries {j, 0}, {j, 1},
  * ... of ceil(n / sca_adamw_chunk_elements()) chunks.  p and g: dtype 0 fp32, 1 bf16, 2 fp16 (computed in fp32, rounded
  * once).  vec = 1 promises that p, g and - with 32-bit states - m, v are aligned to 4 of their elements, and with 8-bit
@@ -379,6 +380,9 @@ typedef struct {
 int sca_adamw_chunk_elements(void);
 int sca_adamw_block_elements(void);
 long long sca_adamw_scratch_bytes(int n_tensors);
+/* Other gradients for the tensors of a table, in the same order: grads [n_tensors] lies in HOST memory and is read before the
+ * call returns.  What vec = 1 promises of g has to hold for the new ones. */
+int sca_adamw_set_grads(sca_adamw_tensor* tensors, int n_tensors, const void* const* grads, void* stream);
 int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_adamw_chunk* chunks, int n_chunks,
                    int state_bits, const float* hyper, long long t, float lr, double beta1, double beta2, float eps,
                    uint64_t seed, void* scratch, void* stream);

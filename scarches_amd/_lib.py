@@ -151,6 +151,7 @@ SIGNATURES = {
     "sca_adamw_chunk_elements": [],
     "sca_adamw_block_elements": [],
     "sca_adamw_scratch_bytes": [I],
+    "sca_adamw_set_grads": [P, I, P, P],
     "sca_adamw_step": [P, I, P, I, I, P, LL, F, D, D, F, U64, P, P],
     "sca_gemm_i8_max_k": [],
     "sca_quant_rows_i8": [P, LL, I, LL, I, P, LL, P, P],

@@ -76,6 +76,15 @@ __global__ __launch_bounds__(256) void adamw_begin_kernel(const AdamWArgs a) {
     a.coef[j] = c;
 }
 
+// New gradients for the tensors of a table: the addresses travel as the launch's arguments, so that nothing on the host has to
+// outlive the call.  (zero_grad() drops the gradients and the next backward pass finds other storage for them, at every step
+// of an ordinary loop; a new table costs 60 us there, this 4.)
+constexpr int PER_LAUNCH = 384;
+struct GradPointers { const void* g[PER_LAUNCH]; };
+__global__ __launch_bounds__(PER_LAUNCH) void adamw_set_grads_kernel(sca_adamw_tensor* tensors, int n, const GradPointers p) {
+    if ((int)threadIdx.x < n) tensors[threadIdx.x].g = p.g[threadIdx.x];
+}
+
 // p of four elements.  denom = sqrt(v) / sqrt(1 - b2^t) + eps; v_sqrt_f32 and v_rcp_f32 are good to one unit in the last
 // place where their arguments are ordinary numbers, the exact sequences (some 25 instructions) are for what is near the
 // denormal ones.
@@ -339,6 +348,19 @@ __global__ __launch_bounds__(256, BITS == 8 ? 6 : 4) void adamw_kernel(const Ada
 extern "C" int sca_adamw_chunk_elements(void) { return CHUNK; }
 extern "C" int sca_adamw_block_elements(void) { return QBLOCK; }
 extern "C" long long sca_adamw_scratch_bytes(int n_tensors) { return n_tensors < 0 ? -1 : (long long)n_tensors * sizeof(Coef); }
+
+extern "C" int sca_adamw_set_grads(sca_adamw_tensor* tensors, int n_tensors, const void* const* grads, void* stream) {
+    if (n_tensors < 0 || (n_tensors > 0 && (!tensors || !grads))) return -1;
+    if (n_tensors == 0) return 0;
+    for (int j = 0; j < n_tensors; j += PER_LAUNCH) {
+        const int n = n_tensors - j < PER_LAUNCH ? n_tensors - j : PER_LAUNCH;
+        GradPointers p = {};
+        for (int i = 0; i < n; ++i) p.g[i] = grads[j + i];
+        hipLaunchKernelGGL(adamw_set_grads_kernel, dim3(1), dim3(PER_LAUNCH), 0, (hipStream_t)stream, tensors + j, n, p);
+    }
+    SCA_CHECK_LAUNCH();
+    return 0;
+}
 
 extern "C" int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_adamw_chunk* chunks,
                               int n_chunks, int state_bits, const float* hyper, long long t, float lr, double beta1,

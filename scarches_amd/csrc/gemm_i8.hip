@@ -40,10 +40,10 @@ struct RowScale {
 };
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// q of VEC values, packed; not for a tiny scale.  x / s + 1.5 * 2^23 in one fma is an integer whose low byte is q in two's complement.  Where one
-// of the values is half a step or more away from its q (a middle, or the estimate fell beside one), all are taken exactly:
-// a branch per vector, seldom taken, instead of a comparison and a choice per value (which bound the kernel: 55 us instead
-// of 29 for 8192 rows of 4096 bf16 values).
+// q of VEC values, packed; not for a tiny scale.  x / s + 1.5 * 2^23 in one fma is an integer whose low byte is q in two's
+// complement.  Where one of the values is half a step or more away from its q (a middle, or the estimate fell beside one),
+// all are taken exactly: a branch per vector, seldom taken, instead of a comparison and a choice per value (which bound the
+// kernel: 55 us instead of 29 for 8192 rows of 4096 bf16 values).
 template <int VEC>
 __device__ __forceinline__ void quantized(const RowScale& sc, const float (&v)[VEC], uint32_t (&w)[VEC / 4]) {
     constexpr float MAGIC = 12582912.f;
@@ -121,36 +121,37 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void quant_rows_kernel(const
 
 // Rows beyond what a workgroup's registers hold: one workgroup per row, read twice (the second time from a cache).
 template <typename T>
-__global__ __launch_bounds__(1024) void quant_rows_long_kernel(const T* __restrict__ x, long long ldx, int k,
-                                                               int8_t* __restrict__ q, long long ldq,
+__global__ __launch_bounds__(1024) void quant_rows_long_kernel(const T* __restrict__ x, long long ldx, long long rows,
+                                                               int k, int8_t* __restrict__ q, long long ldq,
                                                                float* __restrict__ scale) {
     constexpr int VEC = vec_of<T>();
     __shared__ uint32_t scratch[16];
-    const long long r = blockIdx.x;              // (rows this long are fewer than a grid holds)
-    const T* xr = x + r * ldx;
-    int8_t* qr = q + r * ldq;
-    uint32_t amax = 0;
     float v[VEC];
     const int vecs = (k + VEC - 1) / VEC;
-    for (int j = threadIdx.x; j < vecs; j += 1024) {
-        load_vec<T, VEC>(xr + (j * VEC < k - VEC ? j * VEC : k - VEC), v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) amax = magnitude(v[i]) > amax ? magnitude(v[i]) : amax;
-    }
-    const RowScale sc(row_umax<1024>(amax, scratch));
-    if (sc.tiny) {
-        quantize_tiny(xr, k, qr, sc.s, threadIdx.x, 1024);
-    } else {
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+        const T* xr = x + r * ldx;
+        int8_t* qr = q + r * ldq;
+        uint32_t amax = 0;
         for (int j = threadIdx.x; j < vecs; j += 1024) {
-            const int c = j * VEC < k - VEC ? j * VEC : k - VEC;
-            load_vec<T, VEC>(xr + c, v);
-            uint32_t w[VEC / 4];
-            quantized<VEC>(sc, v, w);
-            __builtin_memcpy(qr + c, w, VEC);
+            load_vec<T, VEC>(xr + (j * VEC < k - VEC ? j * VEC : k - VEC), v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) amax = magnitude(v[i]) > amax ? magnitude(v[i]) : amax;
         }
+        const RowScale sc(row_umax<1024>(amax, scratch));
+        if (sc.tiny) {
+            quantize_tiny(xr, k, qr, sc.s, threadIdx.x, 1024);
+        } else {
+            for (int j = threadIdx.x; j < vecs; j += 1024) {
+                const int c = j * VEC < k - VEC ? j * VEC : k - VEC;
+                load_vec<T, VEC>(xr + c, v);
+                uint32_t w[VEC / 4];
+                quantized<VEC>(sc, v, w);
+                __builtin_memcpy(qr + c, w, VEC);
+            }
+        }
+        for (long long c = (long long)k + threadIdx.x; c < ldq; c += 1024) qr[c] = 0;
+        if (threadIdx.x == 0) scale[r] = sc.s;
     }
-    for (long long c = (long long)k + threadIdx.x; c < ldq; c += 1024) qr[c] = 0;
-    if (threadIdx.x == 0) scale[r] = sc.s;
 }
 
 __device__ __forceinline__ i32x4 load16(const int8_t* p, int left) {
@@ -672,8 +673,8 @@ void quant_rows(const void* x, long long ldx, long long rows, int k, int8_t* q, 
     if (vecs <= 2048) QUANT(1024, 2);
     if (vecs <= 4096) QUANT(1024, 4);
 #undef QUANT
-    hipLaunchKernelGGL((quant_rows_long_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, st, (const T*)x, ldx, k, q, ldq,
-                       scale);
+    hipLaunchKernelGGL((quant_rows_long_kernel<T>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(1024), 0,
+                       st, (const T*)x, ldx, rows, k, q, ldq, scale);
 }
 
 template <int BM, int BN, int WM, int WN, int KB, int NS, int KS, bool DIRECT>
@@ -706,7 +707,8 @@ void launch_direct(I8Args a, hipStream_t st) {
 void gemm_i8(const I8Args& a, hipStream_t st) {
     const bool aligned = !(((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.ldx | (uintptr_t)a.ldw) & 15);
     auto tiles = [&](int b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
-    if (a.M <= 16 || (double)a.M * a.N * a.K < 4e8) {
+    const bool fits = ((a.M + 15) / 16) * ((a.N + 15) / 16) < 1 << 23;          // fewer than 2^32 threads
+    if (fits && (a.M <= 16 || (double)a.M * a.N * a.K < 4e8)) {
         launch_direct<int8_t>(a, st);
     } else if (aligned && tiles(256) >= 192 && 16 * tiles(256) <= 5 * tiles(128)) {
         launch_tile<256, 256, 2, 4, 64, 4, 1, true>(a, st);
@@ -719,6 +721,7 @@ void gemm_i8(const I8Args& a, hipStream_t st) {
     }
 }
 
+constexpr int MAX_N = 0x7ffff000;               // (columns are counted in 32 bits, a step of all threads ahead)
 constexpr int I8_MAX_K = (1 << 17) - 1;         // 2^17 products of -128 * -128 would pass int32
 
 void quantize(const void* x, long long ldx, int dtype, long long rows, int k, int8_t* q, long long ldq, float* scale,
@@ -736,7 +739,7 @@ extern "C" int sca_gemm_i8_max_k(void) { return I8_MAX_K; }
 
 extern "C" int sca_quant_rows_i8(const void* x, long long ldx, int dtype, long long rows, int k, int8_t* q,
                                  long long ldq, float* scale, void* stream) {
-    if (dtype < SCA_F32 || dtype > SCA_F16 || rows < 0 || k <= 0 || ldx < 0 || ldq < k) return -1;
+    if (dtype < SCA_F32 || dtype > SCA_F16 || rows < 0 || k <= 0 || k > MAX_N || ldx < 0 || ldq < k) return -1;
     if (rows == 0) return 0;
     if (!x || !q || !scale) return -1;
     quantize(x, ldx, dtype, rows, k, q, ldq, scale, (hipStream_t)stream);
@@ -748,7 +751,7 @@ extern "C" int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, con
                            const float* sw, const void* bias, int btype, long long M, int N, int K, void* y, int ytype,
                            long long ldy, void* stream) {
     if (ytype < SCA_F32 || ytype > SCA_F16 || (btype != SCA_F32 && btype != ytype)) return -1;
-    if (M < 0 || N < 0 || K <= 0 || K > I8_MAX_K || ldx < 0 || ldw < K || ldy < N) return -1;
+    if (M < 0 || N < 0 || N > MAX_N || K <= 0 || K > I8_MAX_K || ldx < 0 || ldw < K || ldy < N) return -1;
     if (M == 0 || N == 0) return 0;
     if (!xq || !sx || !wq || !sw || !y) return -1;
     gemm_i8(I8Args{xq, ldx, sx, wq, ldw, sw, bias, btype, y, ytype, ldy, M, N, K, 0, 0}, (hipStream_t)stream);
@@ -766,7 +769,7 @@ extern "C" int sca_linear_i8(const void* x, long long ldx, int dtype, const int8
                              void* ws, void* stream) {
     if (dtype < SCA_F32 || dtype > SCA_F16 || ytype < SCA_F32 || ytype > SCA_F16) return -1;
     if (btype != SCA_F32 && btype != ytype) return -1;
-    if (M < 0 || N < 0 || K <= 0 || K > I8_MAX_K || ldx < 0 || ldw < K || ldy < N) return -1;
+    if (M < 0 || N < 0 || N > MAX_N || K <= 0 || K > I8_MAX_K || ldx < 0 || ldw < K || ldy < N) return -1;
     if (M == 0 || N == 0) return 0;
     if (!x || !wq || !sw || !y) return -1;
     hipStream_t st = (hipStream_t)stream;

@@ -16,6 +16,7 @@
 
 namespace {
 
+constexpr int MAX_N = 0x7ffff000;                // (columns are counted in 32 bits, a step of all threads ahead)
 constexpr long long MAX_BLOCKS = 1 << 20;        // a launch holds fewer than 2^32 threads; rows beyond it are looped over
 
 // Weight elements [c, c + VEC) of n (type W, so up to 32 bytes), `other` where there is no weight.
@@ -99,40 +100,42 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
                                                            T* __restrict__ y, long long ldy, float* __restrict__ stats) {
     constexpr int VEC = vec_of<T>();
     __shared__ float scratch[16];
-    const long long r = blockIdx.x;              // (rows this long are fewer than a grid holds)
-    const T* xr = x + r * ldx;
     const int vecs = (n + VEC - 1) / VEC;
-    float v[VEC], s = 0.f, q = 0.f;
+    float v[VEC];
     auto col = [&](int j) { return j * VEC < n - VEC ? j * VEC : n - VEC; };
-    for (int j = threadIdx.x; j < vecs; j += 1024) {
-        const int skip = j * VEC - col(j);
-        load_vec<T, VEC>(xr + col(j), v);
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+        const T* xr = x + r * ldx;
+        float s = 0.f, q = 0.f;
+        for (int j = threadIdx.x; j < vecs; j += 1024) {
+            const int skip = j * VEC - col(j);
+            load_vec<T, VEC>(xr + col(j), v);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s += i >= skip ? v[i] : 0.f;
-    }
-    const float mean = row_sum<1024>(s, scratch) / (float)n;
-    for (int j = threadIdx.x; j < vecs; j += 1024) {
-        const int skip = j * VEC - col(j);
-        load_vec<T, VEC>(xr + col(j), v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float d = i >= skip ? v[i] - mean : 0.f;
-            q = fmaf(d, d, q);
+            for (int i = 0; i < VEC; ++i) s += i >= skip ? v[i] : 0.f;
         }
-    }
-    const float rstd = 1.0f / sqrtf(row_sum<1024>(q, scratch) / (float)n + eps);
-    for (int j = threadIdx.x; j < vecs; j += 1024) {
-        float g[VEC], o[VEC];
-        load_weight<ROW_RAGGED>(w, col(j), n, 1.f, g);
-        load_weight<ROW_RAGGED>(b, col(j), n, 0.f, o);
-        load_vec<T, VEC>(xr + col(j), v);
+        const float mean = row_sum<1024>(s, scratch) / (float)n;
+        for (int j = threadIdx.x; j < vecs; j += 1024) {
+            const int skip = j * VEC - col(j);
+            load_vec<T, VEC>(xr + col(j), v);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, g[i], o[i]);
-        store_vec<T, VEC>(y + r * ldy + col(j), v);
-    }
-    if (threadIdx.x == 0 && stats) {
-        stats[r] = mean;
-        stats[rows + r] = rstd;
+            for (int i = 0; i < VEC; ++i) {
+                const float d = i >= skip ? v[i] - mean : 0.f;
+                q = fmaf(d, d, q);
+            }
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<1024>(q, scratch) / (float)n + eps);
+        for (int j = threadIdx.x; j < vecs; j += 1024) {
+            float g[VEC], o[VEC];
+            load_weight<ROW_RAGGED>(w, col(j), n, 1.f, g);
+            load_weight<ROW_RAGGED>(b, col(j), n, 0.f, o);
+            load_vec<T, VEC>(xr + col(j), v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, g[i], o[i]);
+            store_vec<T, VEC>(y + r * ldy + col(j), v);
+        }
+        if (threadIdx.x == 0 && stats) {
+            stats[r] = mean;
+            stats[rows + r] = rstd;
+        }
     }
 }
 
@@ -145,6 +148,7 @@ struct LnBwd {
     const float* stats;
     void* dx; long long lddx;
     float* part;                 // [slab][2][n] partial sums of (dw, db), or null
+    float* means;                // rows beyond the registers: [2][rows]
 };
 
 // NT threads, TPR of them a row.
@@ -254,53 +258,81 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
     put(db, slab + n);
 }
 
-// Rows beyond the registers: one workgroup per row for dx, and columns by slabs of rows for dw and db.
+// Rows beyond the registers (20000 and more genes).  Both operands are read twice: once row by row for the two means, one
+// workgroup per row, and once by columns, for dx and the sums of dw and db together.  (500 x 40000 fp32: LONG_US)
 template <typename T, typename W>
-__global__ __launch_bounds__(1024) void ln_dx_long_kernel(const LnBwd a) {
+__global__ __launch_bounds__(1024) void ln_means_long_kernel(const LnBwd a) {
     constexpr int VEC = vec_of<T>();
     __shared__ float scratch[16];
-    const long long r = blockIdx.x;
     const int n = a.n, vecs = (n + VEC - 1) / VEC;
-    const T *xr = (const T*)a.x + r * a.ldx, *dr = (const T*)a.dy + r * a.lddy;
-    const float mean = a.stats[r], rstd = a.stats[a.rows + r], inv_n = 1.f / (float)n;
-    float h[VEC], d[VEC], g[VEC], s1 = 0.f, s2 = 0.f;
-    auto col = [&](int j) { return j * VEC < n - VEC ? j * VEC : n - VEC; };
-    for (int j = threadIdx.x; j < vecs; j += 1024) {
-        const int skip = j * VEC - col(j);
-        load_vec<T, VEC>(xr + col(j), h);
-        load_vec<T, VEC>(dr + col(j), d);
-        load_weight<ROW_RAGGED>((const W*)a.w, col(j), n, 1.f, g);
+    float h[VEC], d[VEC], g[VEC];
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *xr = (const T*)a.x + r * a.ldx, *dr = (const T*)a.dy + r * a.lddy;
+        const float mean = a.stats[r], rstd = a.stats[a.rows + r];
+        float s1 = 0.f, s2 = 0.f;
+        for (int j = threadIdx.x; j < vecs; j += 1024) {
+            const int c = j * VEC < n - VEC ? j * VEC : n - VEC, skip = j * VEC - c;
+            load_vec<T, VEC>(xr + c, h);
+            load_vec<T, VEC>(dr + c, d);
+            load_weight<ROW_RAGGED>((const W*)a.w, c, n, 1.f, g);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float p = i >= skip ? d[i] * g[i] : 0.f;
-            s1 += p;
-            s2 = fmaf(p, (h[i] - mean) * rstd, s2);
+            for (int i = 0; i < VEC; ++i) {
+                const float p = i >= skip ? d[i] * g[i] : 0.f;
+                s1 += p;
+                s2 = fmaf(p, (h[i] - mean) * rstd, s2);
+            }
+        }
+        s1 = row_sum<1024>(s1, scratch);
+        s2 = row_sum<1024>(s2, scratch);
+        if (threadIdx.x == 0) {
+            a.means[r] = s1 / (float)n;
+            a.means[a.rows + r] = s2 / (float)n;
         }
     }
-    const float m1 = row_sum<1024>(s1, scratch) * inv_n, m2 = row_sum<1024>(s2, scratch) * inv_n;
-    for (int j = threadIdx.x; j < vecs; j += 1024) {
-        load_vec<T, VEC>(xr + col(j), h);
-        load_vec<T, VEC>(dr + col(j), d);
-        load_weight<ROW_RAGGED>((const W*)a.w, col(j), n, 1.f, g);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) d[i] = rstd * (fmaf(d[i], g[i], -m1) - (h[i] - mean) * rstd * m2);
-        store_vec<T, VEC>((T*)a.dx + r * a.lddx + col(j), d);
-    }
 }
-template <typename T>
-__global__ __launch_bounds__(256) void ln_dw_long_kernel(const LnBwd a) {
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= a.n) return;
-    const long long per = (a.rows + gridDim.x - 1) / gridDim.x;
-    const long long r0 = blockIdx.x * per, r1 = r0 + per < a.rows ? r0 + per : a.rows;
-    float sw = 0.f, sb = 0.f;
-    for (long long r = r0; r < r1; ++r) {
-        const float d = to_f32(((const T*)a.dy)[r * a.lddy + c]);
-        sw = fmaf(d, (to_f32(((const T*)a.x)[r * a.ldx + c]) - a.stats[r]) * a.stats[a.rows + r], sw);
-        sb += d;
+// A thread owns the columns of one vector over a slab of rows, four of them in flight.
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void ln_bwd_long_kernel(const LnBwd a) {
+    constexpr int VEC = vec_of<T>(), U = 4;
+    const int n = a.n, slab = blockIdx.y, slabs = gridDim.y;
+    const long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (first >= n) return;
+    const int c = first < n - VEC ? (int)first : n - VEC;
+    const long long r0 = a.rows * slab / slabs, r1 = a.rows * (slab + 1) / slabs;
+    float g[VEC], dw[VEC] = {}, db[VEC] = {};
+    load_weight<ROW_RAGGED>((const W*)a.w, c, n, 1.f, g);
+    for (long long r = r0; r < r1; r += U) {
+        raw_t x[U], dy[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long at = r + u < r1 ? r + u : r1 - 1;
+            load_cols<ROW_RAGGED>((const T*)a.x + at * a.ldx, c, n, x[u]);
+            load_cols<ROW_RAGGED>((const T*)a.dy + at * a.lddy, c, n, dy[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (r + u >= r1) break;
+            const float mean = a.stats[r + u], rstd = a.stats[a.rows + r + u];
+            float h[VEC], d[VEC];
+            unpack<T>(x[u], h);
+            unpack<T>(dy[u], d);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                h[i] = (h[i] - mean) * rstd;
+                dw[i] = fmaf(d[i], h[i], dw[i]);
+                db[i] += d[i];
+            }
+            if (!a.dx) continue;
+            const float m1 = a.means[r + u], m2 = a.means[a.rows + r + u];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) d[i] = rstd * (fmaf(d[i], g[i], -m1) - h[i] * m2);
+            store_vec<T, VEC>((T*)a.dx + (r + u) * a.lddx + c, d);
+        }
     }
-    a.part[(long long)blockIdx.x * 2 * a.n + c] = sw;
-    a.part[(long long)blockIdx.x * 2 * a.n + a.n + c] = sb;
+    if (!a.part) return;
+    float* out = a.part + (long long)slab * 2 * n + c;
+    store_vec<float, VEC>(out, dw);
+    store_vec<float, VEC>(out + n, db);
 }
 
 // dw and db from the slabs: 32 columns per workgroup, 32 threads a column, added in a fixed order.
@@ -327,17 +359,25 @@ __global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restr
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 constexpr int CUS = 256;
+constexpr int MAX_HELD = 16384;                   // longest row of the backward pass in registers
 
 // How the backward pass holds a row of `vecs` vectors: TPR threads, at most 32 elements each (five values are kept per
 // element); 0: not at all.  nt: threads of a workgroup - half as many where there are not enough rows to give every CU
-// eight waves.  slabs: one slab of partial sums per workgroup, which walks the rows: one workgroup per CU.
+// eight waves.  slabs: one slab of partial sums per workgroup, which walks the rows: one workgroup per CU.  Rows that are
+// not held: four workgroups per CU over columns and slabs, and eight rows or more a slab, so that the partial sums stay a
+// small part of what is read.
 struct BwdShape { int tpr, nt, slabs; };
 BwdShape bwd_shape(long long rows, int n, int vec) {
     const int vecs = (n + vec - 1) / vec, v = 32 / vec;
     BwdShape s;
-    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 * v ? 64 : vecs <= 256 * v ? 256 : n <= 16384 ? 1024 : 0;
+    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 * v ? 64 : vecs <= 256 * v ? 256 : n <= MAX_HELD ? 1024 : 0;
     s.nt = s.tpr > 64 ? s.tpr : rows * s.tpr <= 512 * CUS ? 256 : 512;
-    const int per = s.tpr == 0 ? 1 : s.nt / s.tpr;
+    if (s.tpr == 0) {
+        const long long wide = (n + 256LL * vec - 1) / (256LL * vec), want = 4 * CUS / wide, most = (rows + 7) / 8;
+        s.slabs = (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
+        return s;
+    }
+    const int per = s.nt / s.tpr;
     const long long blocks = (rows + per - 1) / per;
     const int most = s.tpr == 256 ? 2 * CUS : CUS;
     s.slabs = (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
@@ -379,7 +419,7 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
     else if (vecs <= 2048) FWD(1024, 2);
     else if (vecs <= 4096) FWD(1024, 4);
     else
-        hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)rows), dim3(1024), 0, st, (const T*)x, ldx, rows, n,
+        hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(1024), 0, st, (const T*)x, ldx, rows, n,
                            (const W*)w, (const W*)b, eps, (T*)y, ldy, stats);
 #undef FWD
 #undef FWD_MODE
@@ -420,9 +460,11 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
 #undef BWD
 #undef BWD_MODE
     } else if (a.rows > 0) {
-        if (a.dx) hipLaunchKernelGGL((ln_dx_long_kernel<T, W>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
-        if (a.part)
-            hipLaunchKernelGGL((ln_dw_long_kernel<T>), dim3(sh.slabs, (n + 255) / 256), dim3(256), 0, st, a);
+        if (a.dx)
+            hipLaunchKernelGGL((ln_means_long_kernel<T, W>), dim3((unsigned)(a.rows < MAX_BLOCKS ? a.rows : MAX_BLOCKS)),
+                               dim3(1024), 0, st, a);
+        hipLaunchKernelGGL((ln_bwd_long_kernel<T, W>), dim3((unsigned)((n + 256LL * VEC - 1) / (256LL * VEC)), sh.slabs),
+                           dim3(256), 0, st, a);
     }
     if (dw || db)
         hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((unsigned)((2LL * n + 31) / 32)), dim3(1024), 0, st, a.part,
@@ -447,25 +489,26 @@ bool ln_types_ok(int dtype, int wtype) {
 extern "C" int sca_layernorm_fwd(const void* x, long long ldx, int dtype, long long rows, int n, const void* w,
                                  const void* b, int wtype, float eps, void* y, long long ldy, float* stats,
                                  void* stream) {
-    if (!ln_types_ok(dtype, wtype) || rows < 0 || n <= 0 || ldx < 0 || ldy < n || !(eps >= 0.f)) return -1;
+    if (!ln_types_ok(dtype, wtype) || rows < 0 || n <= 0 || n > MAX_N || ldx < 0 || ldy < n || !(eps >= 0.f)) return -1;
     if (rows == 0) return 0;
     if (!x || !y) return -1;
     return LN_DISPATCH(ln_fwd, x, ldx, rows, n, w, b, eps, y, ldy, stats, (hipStream_t)stream);
 }
 
 extern "C" long long sca_layernorm_bwd_workspace_floats(long long rows, int n) {
-    if (rows < 0 || n <= 0) return -1;
-    const int a = bwd_shape(rows, n, 4).slabs, b = bwd_shape(rows, n, 8).slabs;      // whatever the type
-    return 2LL * n * (a > b ? a : b);
+    if (rows < 0 || n <= 0 || n > MAX_N) return -1;
+    const BwdShape a = bwd_shape(rows, n, 4), b = bwd_shape(rows, n, 8);             // whatever the type
+    return 2LL * n * (a.slabs > b.slabs ? a.slabs : b.slabs) + (a.tpr && b.tpr ? 0 : 2 * rows);
 }
 
 extern "C" int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, int dtype,
                                  long long rows, int n, const void* w, int wtype, const float* stats, void* dx,
                                  long long lddx, void* dw, void* db, float* ws, void* stream) {
-    if (!ln_types_ok(dtype, wtype) || rows < 0 || n <= 0 || lddy < 0 || ldx < 0 || (dx && lddx < n)) return -1;
+    if (!ln_types_ok(dtype, wtype) || rows < 0 || n <= 0 || n > MAX_N || lddy < 0 || ldx < 0 || (dx && lddx < n)) return -1;
     if (rows > 0 && (!dy || !x || !stats)) return -1;
-    if ((dw || db) && !ws) return -1;
     if (!dx && !dw && !db) return 0;
-    const LnBwd a{dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, dw || db ? ws : nullptr};
+    if (!ws && (dw || db || n > MAX_HELD)) return -1;
+    LnBwd a{dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, dw || db ? ws : nullptr, nullptr};
+    if (n > MAX_HELD) a.means = ws + 2LL * n * bwd_shape(rows, n, dtype == SCA_F32 ? 4 : 8).slabs;
     return LN_DISPATCH(ln_bwd, a, dw, db, (hipStream_t)stream);
 }

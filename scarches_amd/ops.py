@@ -13,6 +13,7 @@ sca_gemm_i8) on the current stream of the tensors' device; there is no CPU fallb
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import numpy as np
@@ -22,6 +23,7 @@ from torch.optim import optimizer as _optimizer
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MAX_WIDTH = 0x7ffff000
 _F8_M, _F8_V = torch.float8_e4m3fn, torch.float8_e5m2
 
 # What a small call costs is its host side (a launch takes 4 us, each allocation 1.5): entry points are looked up once, the
@@ -76,6 +78,11 @@ def _rows(t: torch.Tensor):
     return t, rows, t.stride(0) if rows > 1 else n
 
 
+def _check_width(n):
+    if n > _MAX_WIDTH:
+        raise ValueError(f"rows of {n} values: the kernels count columns in 32 bits, up to {_MAX_WIDTH}")
+
+
 def _like(x):
     """A new contiguous tensor of x's shape and type."""
     return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
@@ -85,6 +92,7 @@ def _like(x):
 def _ln_check(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"layer norm needs a last dimension of at least one value, got shape {tuple(x.shape)}")
+    _check_width(x.shape[-1])
     code = _dtype_code(x, "x")
     if weight is None:
         if bias is not None:
@@ -141,7 +149,7 @@ def layer_norm_bwd(dy, x, weight, stats, need=(True, True, True)):
     dw = torch.empty_like(weight) if need_w else None
     db = torch.empty_like(weight) if need_b else None
     ws = None
-    if need_w or need_b:
+    if need_w or need_b or n > 16384:
         ws = x.new_empty((_fn("sca_layernorm_bwd_workspace_floats")(rows, n),), dtype=torch.float32)
     _call(index, "sca_layernorm_bwd", dy2.data_ptr(), lddy, x2.data_ptr(), ldx, code, rows, n, _lib.ptr(weight), wcode,
           stats.data_ptr(), _lib.ptr(dx), n, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws))
@@ -183,6 +191,7 @@ def quantize_int8(x):
     fastest.  A row of zeros has scale 0; a row with NaN or an infinity has scale NaN, and so have results computed from it."""
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"quantize_int8 needs rows of at least one value, got shape {tuple(x.shape)}")
+    _check_width(x.shape[-1])
     code = _dtype_code(x, "x")
     index = _same_device(x)
     x2, rows, ldx = _rows(x)
@@ -203,6 +212,7 @@ def _i8_check(k, wq, w_scale, bias, out_dtype):
     if wq.dtype != torch.int8 or wq.dim() != 2:
         raise TypeError(f"wq must be an int8 matrix [out, in], not {wq.dtype} {tuple(wq.shape)}")
     n, wk = wq.shape
+    _check_width(n)
     if wk != k or k == 0:
         raise ValueError(f"x has rows of {k} values, wq is {tuple(wq.shape)}")
     if w_scale.dtype != torch.float32 or w_scale.dim() != 1 or w_scale.shape[0] != n or not w_scale.is_contiguous():
@@ -303,8 +313,8 @@ class AdamW(torch.optim.Optimizer):
     the moments of its 256 elements NaN.
 
     The step number of each parameter lies on the device, so `step()` may be captured into a HIP graph after one ordinary
-    call with the same gradients' storage (lr and the other scalars are taken as they are at capture; a graph captured before
-    `load_state_dict` goes on with the states it was captured with).  Gradients have their parameter's type and memory order;
+    call (lr and the other scalars are taken as they are at capture; a graph captured before `load_state_dict` goes on with the
+    states it was captured with; a second graph over gradients in other storage needs an ordinary call in between).  Gradients have their parameter's type and memory order;
     sparse gradients are refused.  One stream at a time may run an optimizer: work that uses it on another stream has to be
     ordered behind the first, as for any tensor."""
 
@@ -329,6 +339,11 @@ class AdamW(torch.optim.Optimizer):
         self._captured = []         # tables (and what they point to) that captured graphs read
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    # Copies and pickles hold the settings, the states and the steps; tables of addresses are made anew.
+    def __getstate__(self):
+        return dict(super().__getstate__(), state_bits=self.state_bits, seed=self.seed, _steps=self._steps,
+                    _host_steps=dict(self._host_steps), _plans={}, _captured=[])
+
     # ------------------------------------------------------------------------------------------ state
     def _check_param(self, p):
         _dtype_code(p, "a parameter")
@@ -346,6 +361,8 @@ class AdamW(torch.optim.Optimizer):
 
     def _init_state(self, p):
         self._check_param(p)
+        if torch.cuda.is_current_stream_capturing():        # zeros that only a replay would write
+            raise RuntimeError("AdamW.step(): a parameter without states; call step() once before the capture")
         st = self.state[p]
         if self.state_bits == 32:
             for k in ("exp_avg", "exp_avg_sq"):
@@ -365,6 +382,8 @@ class AdamW(torch.optim.Optimizer):
 
     def set_step(self, step: int):
         """Set the number of steps that every parameter has behind it (a run taken up from states of another program)."""
+        if int(step) < 0:
+            raise ValueError(f"a parameter cannot have {step} steps behind it")
         for gi in range(len(self.param_groups)):
             self._group_steps(gi).fill_(int(step))
             if self._host_steps.get(gi, 0) is not None:
@@ -403,7 +422,7 @@ class AdamW(torch.optim.Optimizer):
                 self._host_steps[gi] = steps[0] if len(set(steps)) == 1 else None
 
     # ------------------------------------------------------------------------------------------ step
-    def _table(self, gi, group, key):
+    def _table(self, gi, group, key, grads):
         """The device table of a group: entries, chunks, and the tensors that hold them."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step(): the parameters, gradients or states differ from the last call; call it once "
@@ -453,8 +472,8 @@ class AdamW(torch.optim.Optimizer):
         host = torch.from_numpy(np.frombuffer(bytes(size) + entries + chunks.tobytes(), dtype=np.uint8).copy()).pin_memory()
         table = host.to(dev, non_blocking=True)
         at = table.data_ptr() + size
-        return dict(key=key, table=table, streams={_raw_stream(dev.index)}, entries=at, n=len(rows), chunks=at + len(entries),
-                    n_chunks=len(chunks), steps=steps, scratch=table.data_ptr(), index=dev.index)
+        return dict(key=key, grads=grads, captured=False, table=table, streams={_raw_stream(dev.index)}, entries=at,
+                    n=len(rows), chunks=at + len(entries), n_chunks=len(chunks), steps=steps, scratch=table.data_ptr(), index=dev.index)
 
     def _step(self, closure=None):
         loss = None
@@ -464,7 +483,7 @@ class AdamW(torch.optim.Optimizer):
         scales = self.state_bits == 8
         for gi, group in enumerate(self.param_groups):
             # what the table was made of: addresses, sizes, types and layouts
-            key = [group["weight_decay"]]
+            key, grads, bits = [group["weight_decay"]], [], 0
             for p in group["params"]:
                 g = p.grad
                 if g is None:
@@ -473,25 +492,36 @@ class AdamW(torch.optim.Optimizer):
                 st = self.state[p]
                 if not st:
                     self._init_state(p)
-                key += (p.data_ptr(), p.numel(), p.dtype, g.data_ptr(), g.dtype, g.is_contiguous() or g.stride(),
+                at = g.data_ptr()
+                grads.append(at)
+                bits |= at
+                key += (p.data_ptr(), p.numel(), p.dtype, g.dtype, g.is_contiguous() or g.stride(),
                         st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
                 if scales:
                     key += (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr())
-            if len(key) == 1:
+            if not grads:
                 continue
             plan = self._plans.get(gi)
-            if plan is None or plan["key"] != key:
-                plan = self._plans[gi] = self._table(gi, group, key)
+            moved = plan is not None and plan["key"] == key and plan["grads"] != grads
+            if plan is None or plan["key"] != key or moved and (plan["captured"] or bits % 16):
+                plan = self._plans[gi] = self._table(gi, group, key, grads)
+                moved = False
             stream = _raw_stream(plan["index"])
             if stream not in plan["streams"]:
                 plan["streams"].add(stream)
                 if not torch.cuda.is_current_stream_capturing():
                     plan["table"].record_stream(torch.cuda.current_stream(plan["table"].device))
+            if moved:       # gradients in new storage (a graph's table is its own, and stays)
+                _call(plan["index"], "sca_adamw_set_grads", plan["entries"], plan["n"], (ctypes.c_void_p * len(grads))(*grads))
+                plan["grads"] = grads
             # As long as all parameters have taken every step and no graph takes steps that nobody here sees, the step number
             # is given; else the device counts.
             t = self._host_steps.get(gi, 0)
             if torch.cuda.is_current_stream_capturing():    # replays read the table and what it points to
                 self._captured.append((plan, [(p, p.grad, dict(self.state[p])) for p in group["params"]]))
+                plan["captured"] = True
+                if moved:   # the table changes when the graph runs, not now
+                    del self._plans[gi]
                 t = None
             t = self._host_steps[gi] = None if t is None else t + 1
             b1, b2 = group["betas"]

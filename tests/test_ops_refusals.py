@@ -118,3 +118,23 @@ def test_entry_points_check_their_arguments():
         assert lib.sca_adamw_step(*ok[:i], bad, *ok[i + 1:]) == -1, i
     assert lib.sca_adamw_step(a, 1, a, 1, 8, a, 0, 1e-3, 0.9, 0.999, 1e-8, 0, a, None) == -1       # hyper: 32 bits only
     assert lib.sca_adamw_step(a, 1, a, 1, 32, a, 3, 1e-3, 0.9, 0.999, 1e-8, 0, a, None) == -1      # and no step number
+
+
+def test_too_wide():
+    """Columns are counted in 32 bits; a width that would wrap is refused (nothing of that size is allocated here)."""
+    wide = t(1).expand(2 ** 32 + 5)
+    for call in (lambda: ops.layer_norm(wide), lambda: ops.quantize_int8(wide),
+                 lambda: ops.int8_linear(t(4), torch.zeros(1, 1, dtype=I8).expand(2 ** 32 + 5, 4), t(1).expand(2 ** 32 + 5))):
+        with pytest.raises(ValueError):
+            call()
+    lib, a, n = _lib.load(), 1 << 20, 0x7fffffff
+    assert lib.sca_layernorm_fwd(a, n, 0, 1, n, None, None, 0, 1e-5, a, n, a, None) == -1
+    assert lib.sca_layernorm_bwd_workspace_floats(1, n) == -1
+    assert lib.sca_quant_rows_i8(a, n, 0, 1, n, a, n, a, None) == -1
+    assert lib.sca_gemm_i8(a, 4, a, a, 4, a, None, 0, 1, n, 4, a, 0, n, None) == -1
+    # rows beyond the registers need the workspace for dx as well
+    assert lib.sca_layernorm_bwd(a, 16385, a, 16385, 0, 1, 16385, None, 0, a, a, 16385, None, None, None, None) == -1
+    assert lib.sca_adamw_set_grads(None, 1, a, None) == -1 and lib.sca_adamw_set_grads(a, -1, a, None) == -1
+    assert lib.sca_adamw_set_grads(None, 0, None, None) == 0
+    with pytest.raises(ValueError):
+        ops.AdamW([t(3)]).set_step(-1)
