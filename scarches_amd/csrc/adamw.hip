@@ -106,6 +106,19 @@ __device__ __forceinline__ void update(float (&p)[4], const float (&m)[4], const
     for (int k = 0; k < 4; ++k) p[k] = fmaf(-c.step_size, q[k], p[k] * decay);
 }
 
+// Addresses out of a table in memory are of no known kind to the compiler: told that they are device memory it takes the
+// loads and stores for that, whose waits are counted in order.
+template <typename T>
+__device__ __forceinline__ T* global(const void* p) {
+    return (T*)(__attribute__((address_space(1))) T*)(uintptr_t)p;
+}
+
+// What a launch reads only, and every lane alike: through the scalar cache.
+template <typename T>
+__device__ __forceinline__ const T* constant(const T* p) {
+    return (const T*)(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 // ---- 32-bit states ------------------------------------------------------------------------------------------------------
 // 2 x 4 elements of a chunk: all loads first.  28 bytes and some 30 instructions an element (fp32): bound by memory.
 template <typename T>
@@ -116,8 +129,8 @@ __device__ __forceinline__ void chunk32(const sca_adamw_tensor& q, long long i0,
     for (int h = 0; h < 2; ++h) {
         const long long i = i0 + h * 1024, l = q.n - i;
         left[h] = l >= 4 ? 4 : l > 0 ? (int)l : 0;
-        const T *p = (const T*)q.p + i, *g = (const T*)q.g + i;
-        const float *m = (const float*)q.m + i, *v = (const float*)q.v + i;
+        const T *p = global<T>(q.p) + i, *g = global<T>(q.g) + i;
+        const float *m = global<float>(q.m) + i, *v = global<float>(q.v) + i;
         if (q.vec && left[h] == 4) {
             load_vec<T, 4>(p, pv[h]); load_vec<T, 4>(g, gv[h]); load_vec<float, 4>(m, mv[h]); load_vec<float, 4>(v, vv[h]);
         } else {
@@ -136,8 +149,8 @@ __device__ __forceinline__ void chunk32(const sca_adamw_tensor& q, long long i0,
             vv[h][k] = fmaf(a.b2, vv[h][k], a.one_minus_b2 * gk * gk);
         }
         update(pv[h], mv[h], vv[h], c, 1.0f - c.lr * q.weight_decay);
-        T* p = (T*)q.p + i;
-        float *m = (float*)q.m + i, *v = (float*)q.v + i;
+        T* p = global<T>(q.p) + i;
+        float *m = global<float>(q.m) + i, *v = global<float>(q.v) + i;
         if (q.vec && left[h] == 4) {
             store_vec<T, 4>(p, pv[h]); store_vec<float, 4>(m, mv[h]); store_vec<float, 4>(v, vv[h]);
         } else {
@@ -249,12 +262,12 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
     for (int h = 0; h < 2; ++h) {
         const long long i = i0 + h * 1024, l = q.n - i;
         left[h] = l >= 4 ? 4 : l > 0 ? (int)l : 0;
-        const T *p = (const T*)q.p + i, *g = (const T*)q.g + i;
-        const uint8_t *m = (const uint8_t*)q.m + i, *v = (const uint8_t*)q.v + i;
+        const T *p = global<T>(q.p) + i, *g = global<T>(q.g) + i;
+        const uint8_t *m = global<uint8_t>(q.m) + i, *v = global<uint8_t>(q.v) + i;
         // (a wave whose block lies behind the tensor's end has nothing to do, and there is no scale of its block)
         const bool any = (i & ~(long long)(QBLOCK - 1)) < q.n;
-        ms[h] = any ? q.m_scale[i / QBLOCK] : 0.f;
-        vs[h] = any ? q.v_scale[i / QBLOCK] : 0.f;
+        ms[h] = any ? global<float>(q.m_scale)[i / QBLOCK] : 0.f;
+        vs[h] = any ? global<float>(q.v_scale)[i / QBLOCK] : 0.f;
         if (q.vec && left[h] == 4) {
             load_vec<T, 4>(p, pv[h]); load_vec<T, 4>(g, gv[h]);
             mq[h] = *(const uint32_t*)m; vq[h] = *(const uint32_t*)v;
@@ -299,8 +312,8 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
         const uint32_t word[4] = {w.x, w.y, w.z, w.w};
         float msn, vsn;
         const uint32_t mc = to_grid<3, 7, true>(mn, word, msn), vc = to_grid<2, 15, false>(vn, word, vsn);
-        T* p = (T*)q.p + i;
-        uint8_t *m = (uint8_t*)q.m + i, *v = (uint8_t*)q.v + i;
+        T* p = global<T>(q.p) + i;
+        uint8_t *m = global<uint8_t>(q.m) + i, *v = global<uint8_t>(q.v) + i;
         if (q.vec && left[h] == 4) {
             store_vec<T, 4>(p, pv[h]);
             *(uint32_t*)m = mc; *(uint32_t*)v = vc;
@@ -314,8 +327,8 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
                 }
         }
         if ((threadIdx.x & 63) == 0) {
-            q.m_scale[i / QBLOCK] = msn;
-            q.v_scale[i / QBLOCK] = vsn;
+            global<float>(q.m_scale)[i / QBLOCK] = msn;
+            global<float>(q.v_scale)[i / QBLOCK] = vsn;
         }
     }
 }
@@ -324,12 +337,10 @@ __device__ __forceinline__ void chunk8(const sca_adamw_tensor& q, long long i0, 
 // end together.)
 template <int BITS>
 __global__ __launch_bounds__(256, BITS == 8 ? 6 : 4) void adamw_kernel(const AdamWArgs a) {
-    if (!a.coef && blockIdx.x == 0)             // (nothing in this launch reads the steps)
-        for (int j = threadIdx.x; j < a.n_tensors; j += 256) *a.tensors[j].step = a.t;
     for (long long k = blockIdx.x; k < a.n_chunks; k += gridDim.x) {
-        const sca_adamw_chunk ch = a.chunks[k];
-        const sca_adamw_tensor q = a.tensors[ch.tensor];
-        const Coef c = a.coef ? a.coef[ch.tensor] : a.given;
+        const sca_adamw_chunk ch = constant(a.chunks)[k];
+        const sca_adamw_tensor q = constant(a.tensors)[ch.tensor];
+        const Coef c = a.coef ? constant(a.coef)[ch.tensor] : a.given;
         const long long i = (long long)ch.index * CHUNK + 4 * threadIdx.x;
         if (BITS == 32) {
             if (q.dtype == SCA_F32) chunk32<float>(q, i, c, a);
@@ -341,6 +352,8 @@ __global__ __launch_bounds__(256, BITS == 8 ? 6 : 4) void adamw_kernel(const Ada
             else chunk8<sca_f16>(q, i, c, a);
         }
     }
+    if (!a.coef && blockIdx.x == 0)             // (nothing in this launch reads the steps)
+        for (int j = threadIdx.x; j < a.n_tensors; j += 256) *a.tensors[j].step = a.t;
 }
 
 }  // namespace
