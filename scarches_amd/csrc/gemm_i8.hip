@@ -14,36 +14,35 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 namespace {
 
-// q = round(x / s), ties to even, with the exact quotient, for |x| <= 127 s (1 + 2^-23).  The estimate x * (1 / s) may fall
-// on the other side of a middle, so its distance from x is taken without rounding (one fma: q s has at most 31 bits and
-// the difference at most 24).
-__device__ __forceinline__ float nearest(float x, float s, float inv) {
-    float q = rintf(x * inv);
-    const float d = fmaf(-q, s, x), h = 0.5f * s;
-    if (d > h || (d == h && ((int)q & 1))) q += 1.f;
-    else if (d < -h || (d == -h && ((int)q & 1))) q -= 1.f;
-    return q;
-}
-
 // What a row's largest magnitude (as bits: a NaN is above every number) makes of its values.
+//
+// inv: of the two fp32 numbers around 1 / s the one on the same side of 127 / amax as 1 / s itself.  Values of a short type
+// lie half way between two steps of amax / 127 all the time; s, which is that rounded, puts them to one side by the rounding's
+// 2^-24, and an estimate x * inv with that property to the same side.  (With the nearest inv nearly every vector of a bf16
+// row holds a value that has to be corrected.)
 struct RowScale {
     float s, inv, half;
     uint32_t keep;               // 0: a row of zeros, or with a value that is not finite
     bool tiny;                   // 1 / s is not a number of this type: the quotient in 64 bits
-    __device__ __forceinline__ explicit RowScale(uint32_t amax) {
-        s = amax < 0x7f800000u ? __uint_as_float(amax) / 127.f : __uint_as_float(0x7fc00000u);
+    __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+        const float amax = __uint_as_float(bits);
+        s = bits < 0x7f800000u ? amax / 127.f : __uint_as_float(0x7fc00000u);
         keep = s > 0.f ? 0xffffffffu : 0u;
         tiny = s > 0.f && s < 1e-37f;
         inv = keep ? 1.f / s : 0.f;
         half = 0.5f * s;
+        const float side = fmaf(-127.f, s, amax), got = fmaf(inv, amax, -127.f);       // (one rounding each: exact signs)
+        if (keep && side > 0.f && !(got > 0.f)) inv = __uint_as_float(__float_as_uint(inv) + 1u);
+        if (keep && side < 0.f && !(got < 0.f)) inv = __uint_as_float(__float_as_uint(inv) - 1u);
     }
 };
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// q of VEC values, packed; not for a tiny scale.  x / s + 1.5 * 2^23 in one fma is an integer whose low byte is q in two's
-// complement.  Where one of the values is half a step or more away from its q (a middle, or the estimate fell beside one),
-// all are taken exactly: a branch per vector, seldom taken, instead of a comparison and a choice per value (which bound the
-// kernel: 55 us instead of 29 for 8192 rows of 4096 bf16 values).
+// q = round(x / s) of VEC values, ties to even, with the exact quotient, packed; not for a tiny scale.  x / s + 1.5 * 2^23 in
+// one fma is an integer whose low byte is q in two's complement.  The estimate may fall on the other side of a middle, so its
+// distance from x is taken without rounding (one fma: q s has at most 31 bits and the difference at most 24), and where one
+// of the values is half a step or more away from its q, all are put right: a branch per vector, seldom taken.  (8192 rows
+// of 4096 bf16 values: 18 us, the rate of a copy; a comparison and a choice for every value takes 55.)
 template <int VEC>
 __device__ __forceinline__ void quantized(const RowScale& sc, const float (&v)[VEC], uint32_t (&w)[VEC / 4]) {
     constexpr float MAGIC = 12582912.f;
@@ -55,7 +54,11 @@ __device__ __forceinline__ void quantized(const RowScale& sc, const float (&v)[V
     }
     if (far >= sc.half) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) t[i] = nearest(v[i], sc.s, sc.inv) + MAGIC;
+        for (int i = 0; i < VEC; ++i) {
+            // beyond half a step, or at it with an odd q: the neighbour.  (|d| + the last bit of q, as integers, > half)
+            const float d = fmaf(-(t[i] - MAGIC), sc.s, v[i]);
+            if (magnitude(d) + (__float_as_uint(t[i]) & 1u) > __float_as_uint(sc.half)) t[i] += copysignf(1.f, d);
+        }
     }
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
 }
 
 // Rows beyond the registers (20000 and more genes).  Both operands are read twice: once row by row for the two means, one
-// workgroup per row, and once by columns, for dx and the sums of dw and db together.  (500 x 40000 fp32: LONG_US)
+// workgroup per row, and once by columns, for dx and the sums of dw and db together.  (500 x 40000 fp32: 71 us, 3.4 TB/s by the three arrays.)
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_means_long_kernel(const LnBwd a) {
     constexpr int VEC = vec_of<T>();
