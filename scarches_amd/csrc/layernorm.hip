@@ -186,16 +186,19 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
     // 16-bit rows, whose arithmetic takes half as long as their loads: the next row is on its way meanwhile (16384 x 4000
     // bf16: 81 instead of 100 us).  fp32 rows have no registers for it and run at the rate of a copy without.
     constexpr bool AHEAD = sizeof(T) == 2;
+    // (where rows meet at barriers, a wave without a row of its own goes along with zeros)
+    constexpr bool TOGETHER = PER > 1 && TPR > 64;
     long long r = (long long)blockIdx.x * PER + sub;
     if (AHEAD && r < a.rows) load(r);
-    for (; r < a.rows; r += step) {
-        if (!AHEAD) load(r);
+    for (; (TOGETHER ? r - sub : r) < a.rows; r += step) {
+        const bool mine = !TOGETHER || r < a.rows;
+        if (!AHEAD && mine) load(r);
         raw_t x0[V], d0[V];
-        const float mean0 = mean, rstd0 = rstd;
+        const float mean0 = mine ? mean : 0.f, rstd0 = mine ? rstd : 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            x0[j] = xq[j];
-            d0[j] = dq[j];
+            x0[j] = mine ? xq[j] : raw_t{0, 0, 0, 0};
+            d0[j] = mine ? dq[j] : raw_t{0, 0, 0, 0};
         }
         if (AHEAD && r + step < a.rows) load(r + step);
         float s1 = 0.f, s2 = 0.f, h[VEC], d[VEC];
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const Cols<T, TPR, MODE> at(j, t, n);
-            if (!at.there) continue;
+            if (!at.there || !mine) continue;
             unpack_again<T>(x0[j], h);
             unpack_again<T>(d0[j], d);
 #pragma unroll
@@ -259,7 +262,8 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
 }
 
 // Rows beyond the registers (20000 and more genes).  Both operands are read twice: once row by row for the two means, one
-// workgroup per row, and once by columns, for dx and the sums of dw and db together.  (500 x 40000 fp32: 71 us, 3.4 TB/s by the three arrays.)
+// workgroup per row, and once by columns, for dx and the sums of dw and db together.  (500 x 40000 fp32:
+// 71 us, 3.4 TB/s by the three arrays.)
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_means_long_kernel(const LnBwd a) {
     constexpr int VEC = vec_of<T>();
@@ -363,15 +367,19 @@ constexpr int MAX_HELD = 16384;                   // longest row of the backward
 
 // How the backward pass holds a row of `vecs` vectors: TPR threads, at most 32 elements each (five values are kept per
 // element); 0: not at all.  nt: threads of a workgroup - half as many where there are not enough rows to give every CU
-// eight waves.  slabs: one slab of partial sums per workgroup, which walks the rows: one workgroup per CU.  Rows that are
-// not held: four workgroups per CU over columns and slabs, and eight rows or more a slab, so that the partial sums stay a
-// small part of what is read.
+// eight waves.  Four waves a row and four rows a workgroup (us of one wave a row / this; 1000, 2000, 8000 rows): fp32 of 493
+// vectors 15.0 / 12.4, 18.5 / 15.1, 38.3 / 35.1; of 251 vectors 10.4 / 9.6, 11.7 / 9.7, 21.9 / 22.8; fp16 of 126 vectors
+// 10.1 / 10.6, 9.6 / 11.0, 15.3 / 22.2.
+// slabs: one slab of partial sums per workgroup, which walks the rows: one workgroup per CU.  Rows that are not held: four
+// workgroups per CU over columns and slabs, and eight rows or more a slab, so that the partial sums stay a small part of
+// what is read.
 struct BwdShape { int tpr, nt, slabs; };
 BwdShape bwd_shape(long long rows, int n, int vec) {
     const int vecs = (n + vec - 1) / vec, v = 32 / vec;
     BwdShape s;
-    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 * v ? 64 : vecs <= 256 * v ? 256 : n <= MAX_HELD ? 1024 : 0;
-    s.nt = s.tpr > 64 ? s.tpr : rows * s.tpr <= 512 * CUS ? 256 : 512;
+    const bool four = vecs > 128 && vecs <= 512 && (vecs > 256 || rows <= 8 * CUS);
+    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 && !four ? 64 : vecs <= 256 * v ? 256 : n <= MAX_HELD ? 1024 : 0;
+    s.nt = four ? 1024 : s.tpr > 64 ? s.tpr : rows * s.tpr <= 512 * CUS ? 256 : 512;
     if (s.tpr == 0) {
         const long long wide = (n + 256LL * vec - 1) / (256LL * vec), want = 4 * CUS / wide, most = (rows + 7) / 8;
         s.slabs = (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
@@ -379,7 +387,7 @@ BwdShape bwd_shape(long long rows, int n, int vec) {
     }
     const int per = s.nt / s.tpr;
     const long long blocks = (rows + per - 1) / per;
-    const int most = s.tpr == 256 ? 2 * CUS : CUS;
+    const int most = s.nt == 256 && s.tpr == 256 ? 2 * CUS : CUS;
     s.slabs = (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
     return s;
 }
@@ -445,15 +453,16 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
         if (sh.nt == 256) BWD(TPR, V, 256); \
         else BWD(TPR, V, 512);              \
     } while (0)
-        if (mode == ROW_TINY && sh.nt == 256) BWD_MODE(4, 1, ROW_TINY, 256);
+        if (sh.nt > sh.tpr && sh.tpr == 256 && vecs <= 256) BWD(256, 1, 1024);
+        else if (sh.nt > sh.tpr && sh.tpr == 256) BWD(256, 2, 1024);
+        else if (mode == ROW_TINY && sh.nt == 256) BWD_MODE(4, 1, ROW_TINY, 256);
         else if (mode == ROW_TINY) BWD_MODE(4, 1, ROW_TINY, 512);
         else if (vecs <= 4) BWD2(4, 1);
         else if (vecs <= 16) BWD2(16, 1);
         else if (vecs <= 32) BWD2(32, 1);
         else if (vecs <= 64) BWD2(64, 1);
         else if (vecs <= 64 * 2) BWD2(64, 2);
-        else if (V > 4 && vecs <= 64 * 4) BWD2(64, (V > 4 ? 4 : V));
-        else if (vecs <= 64 * V) BWD2(64, V);
+        else if (vecs <= 64 * 4) BWD2(64, 4);
         else if (vecs <= 256 * V) BWD(256, V, 256);
         else BWD(1024, V / 2, 1024);
 #undef BWD2

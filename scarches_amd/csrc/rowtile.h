@@ -86,8 +86,8 @@ __device__ __forceinline__ void store_cols(T* __restrict__ row, int c, int n, co
     else store_vec<T, VEC>(row + c, v);
 }
 
-// Sum / integer maximum over the TPR threads of a row, in every one of them.  TPR > 64: the row is the workgroup's, and
-// `scratch` (one entry per wave) is LDS that nothing else uses until the next barrier.
+// Sum / integer maximum over the TPR threads of a row, in every one of them.  TPR > 64: all threads of the workgroup call it
+// together, and `scratch` (one entry per wave) is LDS that nothing else uses until the next barrier.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* scratch) {
     if constexpr (TPR >= 64) v = wave_sum(v);
@@ -105,7 +105,7 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
         __syncthreads();
         v = 0.f;
 #pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) v += scratch[i];
+        for (int i = 0; i < TPR / 64; ++i) v += scratch[threadIdx.x / TPR * (TPR / 64) + i];
     }
     return v;
 }
@@ -122,7 +122,10 @@ __device__ __forceinline__ uint32_t row_umax(uint32_t v, uint32_t* scratch) {
         __syncthreads();
         v = 0;
 #pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) v = scratch[i] > v ? scratch[i] : v;
+        for (int i = 0; i < TPR / 64; ++i) {
+            const uint32_t b = scratch[threadIdx.x / TPR * (TPR / 64) + i];
+            v = b > v ? b : v;
+        }
     }
     return v;
 }
