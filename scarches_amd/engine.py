@@ -689,8 +689,8 @@ class CVAEEngine:
                     if (lane, other) in self._side_deps and torch.cuda.is_current_stream_capturing():
                         # ROCm 7.2: hipStreamEndCapture segfaults when two FORKED streams of one capture wait for each
                         # other in both directions (A waits for an event of B after B waited for one of A - acyclic and
-                        # legal; torch-only reproduction in scripts/dbg/capture_crash_repro.py, also through a third
-                        # stream, also without work in between).  The second direction goes through the origin stream.
+                        # legal; also through a third stream, also without work in between).  The second direction goes
+                        # through the origin stream.
                         main = torch.cuda.current_stream(self.device)
                         ev3 = self._next_event()
                         self._call(main.wait_event, ev2)
