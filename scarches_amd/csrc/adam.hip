@@ -135,7 +135,7 @@ extern "C" int sca_begin_step(float* hyper, uint32_t* step_ctr, float alpha_kl, 
 
 extern "C" int sca_fill_zero(void* p, long long bytes, void* stream) {
     if (bytes <= 0) return 0;
-    hipError_t e = hipMemsetAsync(p, 0, (size_t)bytes, (hipStream_t)stream);
+    hipError_t e = fill_zero(p, (size_t)bytes, (hipStream_t)stream);
     return e == hipSuccess ? 0 : (int)e;
 }
 

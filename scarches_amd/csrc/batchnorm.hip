@@ -154,7 +154,7 @@ extern "C" int sca_bn_fwd(float* a, int B, int H, const float* gamma, const floa
     if (B <= 0 || H <= 0) return 0;
     hipStream_t st = (hipStream_t)stream;
     if (use_batch_stats) {
-        hipError_t e = hipMemsetAsync(acc, 0, sizeof(double) * 2 * (size_t)H, st);
+        hipError_t e = fill_zero(acc, sizeof(double) * 2 * (size_t)H, st);
         if (e != hipSuccess) return (int)e;
         hipLaunchKernelGGL(bn_colstats_kernel, dim3((H + 63) / 64, (B + BN_ROWS - 1) / BN_ROWS), dim3(256), 0, st, a,
                            B, H, acc);
@@ -174,7 +174,7 @@ extern "C" int sca_bn_bwd(const float* dh, int S, long long slab_stride, const f
                           const uint32_t* step, double* acc, float* da, float* dgamma, float* dbeta, void* stream) {
     if (B <= 0 || H <= 0) return 0;
     hipStream_t st = (hipStream_t)stream;
-    hipError_t e = hipMemsetAsync(acc, 0, sizeof(double) * 2 * (size_t)H, st);
+    hipError_t e = fill_zero(acc, sizeof(double) * 2 * (size_t)H, st);
     if (e != hipSuccess) return (int)e;
     BnBwdArgs a{dh, S, slab_stride, extra, B, H, xhat, stats, gamma, beta, p, mask, seed, rng_stream, step, da, acc,
                 dgamma, dbeta};

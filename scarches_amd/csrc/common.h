@@ -11,6 +11,24 @@
         if (e__ != hipSuccess) return (int)e__;              \
     } while (0)
 
+// ----------------------------------------------------------------------------- zeroing
+// By a kernel: memory-set nodes of captured graphs have given wrong results on replays after the first.
+static __global__ __launch_bounds__(256) void fill_zero_kernel(uint8_t* p, long long bytes) {
+    const long long head = (16 - ((uintptr_t)p & 15)) & 15, i0 = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long step = (long long)gridDim.x * 256, words = bytes > head ? (bytes - head) / 16 : 0;
+    for (long long i = i0; i < words; i += step) ((uint4*)(p + head))[i] = uint4{0, 0, 0, 0};
+    if (i0 < head && i0 < bytes) p[i0] = 0;
+    const long long tail = head + words * 16 + i0;
+    if (i0 < 16 && tail < bytes) p[tail] = 0;
+}
+inline hipError_t fill_zero(void* p, size_t bytes, hipStream_t st) {
+    if (bytes == 0) return hipSuccess;
+    const size_t blocks = (bytes + 4095) / 4096;
+    hipLaunchKernelGGL(fill_zero_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, (uint8_t*)p,
+                       (long long)bytes);
+    return hipGetLastError();
+}
+
 // ----------------------------------------------------------------------------- reductions
 // Wave-wide (64 lanes) reductions, result in every lane.  Within a row of 16 lanes: four DPP steps (quad_perm xor 1,
 // xor 2, row_half_mirror, row_mirror - no LDS round trip, no lane-address arithmetic); across the four rows: the row

@@ -362,12 +362,12 @@ extern "C" int sca_layer_bwd(const float* dh, int S, long long slab_stride, cons
     return 0;
 }
 
-// segT must hold max(C,1)*H floats; it is zeroed here (memset node), filled by atomics, then finished.
+// segT must hold max(C,1)*H floats; it is zeroed here, filled by atomics, then finished.
 extern "C" int sca_cond_colsum(const float* da, int B, int H, const int32_t* cond, int C, float* segT, float* dWc,
                                float* db, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     const int Cs = (cond && C > 0) ? C : 1;
-    hipError_t e = hipMemsetAsync(segT, 0, (size_t)Cs * H * sizeof(float), st);
+    hipError_t e = fill_zero(segT, (size_t)Cs * H * sizeof(float), st);
     if (e != hipSuccess) return (int)e;
     if (B > 0) {
         dim3 grid((B + COLSUM_ROWS - 1) / COLSUM_ROWS, (H + 255) / 256);

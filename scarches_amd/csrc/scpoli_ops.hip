@@ -292,7 +292,7 @@ extern "C" int sca_proto_loss(const float* z, int ld, int B, int Z, const float*
     float* mind = (float*)(assign + B);
     float* rl = mind + B;
     float* ru = rl + B;
-    hipError_t e = hipMemsetAsync(cnt, 0, sizeof(int) * (size_t)(K + Ku), st);
+    hipError_t e = fill_zero(cnt, sizeof(int) * (size_t)(K + Ku), st);
     if (e != hipSuccess) return (int)e;
     ProtoArgs a{z, ld, B, Z, P, K, labels, n_levels, labeled, Pu, Ku, cnt, assign, mind, rl, ru, weight, weight_u,
                 dz, lddz, dPu};
