@@ -391,6 +391,9 @@ int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_ada
  * sca_quant_rows_i8: scale[r] = max_k |x_rk| / 127, q_rk = round(x_rk / scale[r]) (ties to even, the exact quotient), and
  * q_rk = 0 for k <= column < ldq.  x: dtype 0 fp32, 1 bf16, 2 fp16, rows of pitch ldx.  A row of zeros has scale 0; a row
  * with a value that is not finite has scale NaN and q = 0, so that what is computed from it is NaN.
+ * sca_csr_quant_rows_i8: the same of rows row_ids[b] (NULL: 0 ... B-1) of a canonical CSR matrix of G columns, of log(1 + x)
+ * with apply_log1p: bit for bit what sca_csr_gather_rows followed by sca_quant_rows_i8 gives.  q: 16-byte aligned, ldq a
+ * multiple of 16; -2 when ldq > 65536 (the row is put together in LDS; the caller takes the other two then).
  * sca_gemm_i8: y[m][n] = (sum_k xq[m][k] wq[n][k]) * sx[m] * sw[n] + bias[n], the sum exact in int32 (K <=
  * sca_gemm_i8_max_k()), the rest in fp32, rounded once to ytype.  wq is a torch Linear weight [N][K] in int8 with pitch ldw.
  * bias (may be NULL): btype 0 or ytype.  Any pitches and alignments; 16-byte aligned operands whose pitch is a multiple of
@@ -402,6 +405,8 @@ int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_ada
 int sca_gemm_i8_max_k(void);
 int sca_quant_rows_i8(const void* x, long long ldx, int dtype, long long rows, int k, int8_t* q, long long ldq,
                       float* scale, void* stream);
+int sca_csr_quant_rows_i8(const int64_t* indptr, const int32_t* indices, const float* data, const int64_t* row_ids, int B,
+                          int G, int apply_log1p, int8_t* q, int ldq, float* scale, void* stream);
 int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, const int8_t* wq, long long ldw, const float* sw,
                 const void* bias, int btype, long long M, int N, int K, void* y, int ytype, long long ldy, void* stream);
 long long sca_linear_i8_workspace_bytes(long long M, int K);

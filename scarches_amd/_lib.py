@@ -155,6 +155,7 @@ SIGNATURES = {
     "sca_adamw_step": [P, I, P, I, I, P, LL, F, D, D, F, U64, P, P],
     "sca_gemm_i8_max_k": [],
     "sca_quant_rows_i8": [P, LL, I, LL, I, P, LL, P, P],
+    "sca_csr_quant_rows_i8": [P, P, P, P, I, I, I, P, I, P, P],
     "sca_gemm_i8": [P, LL, P, P, LL, P, P, I, LL, I, I, P, I, LL, P],
     "sca_linear_i8_workspace_bytes": [LL, I],
     "sca_linear_i8": [P, LL, I, P, LL, P, P, I, LL, I, I, P, I, LL, P, P],

@@ -2196,18 +2196,37 @@ class CVAEEngine:
 
     def _first_product(self, a, B, st, int8, max_split=None):
         """x W0^T of the first encoder layer as (ptr, slabs, stride): fp32, or in 8-bit integers with one scale per cell
-        and per output (`int8` = quantize_first_layer())."""
+        and per output (`int8` = quantize_first_layer()).  a: the cells as fp32 rows, or what `_quantized_cells` returned."""
         ly = self.enc[0]
         if int8 is None:
             return self._gemm(0, 0, a, ly.n_in, self.p[ly.w].data_ptr(), ly.n_in, B, ly.n_out, ly.n_in, st,
                               max_split=max_split)
         wq, scale = int8
         raw, slab = self.lib._lib, self.ws["slab"]
+        if isinstance(a, tuple):
+            q, sx = a
+            _lib.check(raw.sca_gemm_i8(q.data_ptr(), q.stride(0), sx.data_ptr(), wq.data_ptr(), wq.stride(0), scale.data_ptr(),
+                                       None, 0, B, ly.n_out, ly.n_in, slab.data_ptr(), 0, ly.n_out, st), "gemm_i8")
+            return slab.data_ptr(), 1, B * ly.n_out
         size = raw.sca_linear_i8_workspace_bytes(B, ly.n_in)
         scratch = torch.empty(size, dtype=torch.int8, device=self.device) if size else None
         _lib.check(raw.sca_linear_i8(a, ly.n_in, 0, wq.data_ptr(), wq.stride(0), scale.data_ptr(), None, 0, B, ly.n_out,
                                      ly.n_in, slab.data_ptr(), 0, ly.n_out, _lib.ptr(scratch), st), "linear_i8")
         return slab.data_ptr(), 1, B * ly.n_out
+
+    def _quantized_cells(self, row_ids, B, log1p, st):
+        """(q, scale): rows of the bound CSR matrix in 8-bit integers, without their fp32 rows in between; None where the
+        kernel does not take rows this wide."""
+        ip, ix, dv = self.csr
+        pitch = -(-self.G // 128) * 128
+        q = torch.empty((B, pitch), dtype=torch.int8, device=self.device)
+        scale = torch.empty((B,), dtype=torch.float32, device=self.device)
+        rc = self.lib._lib.sca_csr_quant_rows_i8(ip.data_ptr(), ix.data_ptr(), dv.data_ptr(), _lib.ptr(row_ids), B, self.G, log1p,
+                                                 q.data_ptr(), pitch, scale.data_ptr(), st)
+        if rc == -2:
+            return None
+        _lib.check(rc, "csr_quant_rows_i8")
+        return q, scale
 
     def encode(self, row_ids, cond, B, mean=True, x_dense=None, eps=None, covs=None, int8=None):
         """Eval-mode encoder pass: returns (z or mean [B,Z], mean, var) device tensors (views of the workspace).
@@ -2221,14 +2240,16 @@ class CVAEEngine:
         ptr = _lib.ptr
         G, C, Z = self.G, self.C, self.Zt
         log1p = 0 if self.recon == "mse" else 1
-        if x_dense is not None:
-            _lib.check(L.sca_dense_gather_rows(ptr(x_dense), x_dense.stride(0), ptr(row_ids), B, G, log1p,
-                                               ws["x"].data_ptr(), G, ws["sf"].data_ptr(), st), "dense_gather")
-        else:
-            ip, ix, dv = self.csr
-            _lib.check(L.sca_csr_gather_rows(ip.data_ptr(), ix.data_ptr(), dv.data_ptr(), ptr(row_ids), B, G, log1p,
-                                             ws["x"].data_ptr(), G, ws["sf"].data_ptr(), st), "csr_gather")
-        a = ws["x"].data_ptr()
+        a = self._quantized_cells(row_ids, B, log1p, st) if int8 is not None and x_dense is None else None
+        if a is None:
+            if x_dense is not None:
+                _lib.check(L.sca_dense_gather_rows(ptr(x_dense), x_dense.stride(0), ptr(row_ids), B, G, log1p,
+                                                   ws["x"].data_ptr(), G, ws["sf"].data_ptr(), st), "dense_gather")
+            else:
+                ip, ix, dv = self.csr
+                _lib.check(L.sca_csr_gather_rows(ip.data_ptr(), ix.data_ptr(), dv.data_ptr(), ptr(row_ids), B, G, log1p,
+                                                 ws["x"].data_ptr(), G, ws["sf"].data_ptr(), st), "csr_gather")
+            a = ws["x"].data_ptr()
         cond_p = ptr(cond) if C > 0 else None
         if self.use_fused_mid and not self.cond_embed and os.environ.get("SCA_ENCODE_FUSED", "1") == "1":
             # first-layer GEMM, then ONE launch for its epilogue, the remaining encoder layers, the heads and the latent

@@ -117,6 +117,7 @@ def test_latent_in_8_bit_integers(hidden, use_bn):
     mu = torch.from_numpy(m.get_latent(mean=True, int8=True)).cuda()
     eng.noise_off = True
     assert m.get_latent(int8=True).shape == (500, 6) and len(m.get_latent(mean_var=True, int8=True)) == 2
+    m.get_latent(mean=True)                 # leaves the gathered cells in the workspace
     x = eng.ws["x"][:500 * 197].view(-1)[:500 * 197].view(500, 197) if eng.ws["x"].dim() == 1 else eng.ws["x"][:500]
     ly = eng.enc[0]
     wq, ws = eng.quantize_first_layer()
@@ -144,3 +145,37 @@ def test_latent_in_8_bit_integers(hidden, use_bn):
     assert (mu.double() - ref).abs().max() <= 1e-5 * max(1.0, ref.abs().max().item())
     exact = torch.from_numpy(m.get_latent(mean=True)).cuda()
     assert not torch.equal(exact, mu)
+
+
+@pytest.mark.parametrize("G,nnz,log1p", [(197, 40, 1), (2000, 284, 1), (2000, 1999, 0), (15, 3, 1), (20011, 900, 1), (65536, 70, 0)])
+def test_csr_rows_in_8_bit_integers(G, nnz, log1p):
+    """Rows of a CSR matrix, quantized on the way: bit for bit the gather followed by the row quantization - empty rows, stored
+    zeros, unsorted columns, repeated and permuted rows, values that are not finite, a scale below what fp32 inverts."""
+    from scarches_amd import _lib, ops
+    lib = _lib.load()
+    g = np.random.default_rng(G + nnz)
+    counts = g.integers(0, nnz + 1, 37)
+    counts[[0, 5]] = 0
+    counts[1] = nnz
+    indptr = np.concatenate([[0], np.cumsum(counts)]).astype(np.int64)
+    indices = np.concatenate([g.permutation(G)[:c] for c in counts]).astype(np.int32)
+    data = (g.integers(0, 60, indptr[-1]) if log1p else g.standard_normal(indptr[-1])).astype(np.float32)
+    if log1p == 0:
+        data[indptr[2]:indptr[3]] *= np.float32(1e-38)
+        data[indptr[3]:indptr[3] + 1] = np.nan
+        data[indptr[4]:indptr[4] + 1] = np.inf
+    ip, ix, dv = (torch.from_numpy(t).cuda() for t in (indptr, indices, data))
+    for rows in (None, torch.from_numpy(g.integers(0, 37, 300)).cuda()):
+        B = 37 if rows is None else 300
+        x = torch.empty(B, G, device="cuda")
+        st = torch.cuda.current_stream().cuda_stream
+        _lib.check(lib.sca_csr_gather_rows(ip.data_ptr(), ix.data_ptr(), dv.data_ptr(), _lib.ptr(rows), B, G, log1p, x.data_ptr(),
+                                           G, torch.empty(B, device="cuda").data_ptr(), st), "gather")
+        want, scale = ops.quantize_int8(x)
+        pitch = -(-G // 128) * 128
+        q = torch.full((B + 1, pitch), 77, dtype=torch.int8, device="cuda")
+        s = torch.empty(B, device="cuda")
+        _lib.check(lib.sca_csr_quant_rows_i8(ip.data_ptr(), ix.data_ptr(), dv.data_ptr(), _lib.ptr(rows), B, G, log1p,
+                                             q.data_ptr(), pitch, s.data_ptr(), st), "csr_quant_rows_i8")
+        assert torch.equal(q[:B, :G], want) and torch.equal(s.view(torch.int32), scale.view(torch.int32))
+        assert not q[:B, G:].any() and (q[B] == 77).all()               # padded with zeros; the row behind is left alone

@@ -138,3 +138,12 @@ def test_too_wide():
     assert lib.sca_adamw_set_grads(None, 0, None, None) == 0
     with pytest.raises(ValueError):
         ops.AdamW([t(3)]).set_step(-1)
+
+
+def test_csr_rows_entry_point():
+    lib, a = _lib.load(), 1 << 20
+    ok = (a, a, a, None, 4, 100, 1, a, 112, a, None)
+    for i, bad in ((0, None), (1, None), (2, None), (4, -1), (5, 0), (7, None), (7, a + 4), (8, 96), (8, 100), (9, None)):
+        assert lib.sca_csr_quant_rows_i8(*ok[:i], bad, *ok[i + 1:]) == -1, i
+    assert lib.sca_csr_quant_rows_i8(a, a, a, None, 4, 65537, 1, a, 65552, a, None) == -2       # wider than the LDS
+    assert lib.sca_csr_quant_rows_i8(a, a, a, None, 0, 100, 1, a, 112, a, None) == 0
