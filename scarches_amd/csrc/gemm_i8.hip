@@ -159,7 +159,7 @@ __global__ __launch_bounds__(1024) void quant_rows_long_kernel(const T* __restri
 
 // Rows of a CSR matrix (canonical: one entry per row and column), log(1 + x) on the way: what sca_csr_gather_rows and
 // quant_rows_kernel give, without the dense fp32 rows between them, nearly all of which are zeros (8192 cells of 284 stored
-// counts in 2000 genes: CSR_US us instead of 19 + 13.6).  One wave per row, which is put together in LDS; the first HELD stored
+// counts in 2000 genes: 14 us instead of 17 + 13.6).  One wave per row, which is put together in LDS; the first HELD stored
 // values of a lane stay in registers between the maximum and the quotients, what is beyond them is read again.
 constexpr int CSR_LDS = 65536;
 
@@ -171,7 +171,8 @@ __global__ __launch_bounds__(64) void csr_quant_rows_kernel(const int64_t* __res
     extern __shared__ __attribute__((aligned(16))) int8_t row[];
     constexpr int HELD = 8;
     const long long b = blockIdx.x, r = row_ids ? row_ids[b] : b;
-    const int64_t s = indptr[r] + threadIdx.x, e = indptr[r + 1];
+    const int64_t first = indptr[r], s = first + threadIdx.x, e = indptr[r + 1];
+    const int held = e - first >= HELD * 64 ? HELD : (int)((e - first + 63) / 64);      // (the logarithms are what it waits for)
     float v[HELD];
     int g[HELD];
     uint32_t amax = 0;
@@ -184,6 +185,7 @@ __global__ __launch_bounds__(64) void csr_quant_rows_kernel(const int64_t* __res
     for (int c = threadIdx.x * 16; c < ldq; c += 1024) *(i32x4*)(row + c) = i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < HELD; ++j) {
+        if (j >= held) break;
         if (log1p) v[j] = log1pf(v[j]);
         amax = magnitude(v[j]) > amax ? magnitude(v[j]) : amax;
     }
@@ -204,6 +206,7 @@ __global__ __launch_bounds__(64) void csr_quant_rows_kernel(const int64_t* __res
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < HELD; j += 4) {
+        if (j >= held) break;
         const float x[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
         put(x, g + j);
     }
