@@ -334,7 +334,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 8 or 32, not {state_bits}")
         self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFFFFFFFFFF
         self._steps = {}            # group number -> int64 [parameters] on the device: their steps
-        self._host_steps = {}       # group number -> the step of all its parameters, None where only the device knows
+        # group number -> (the step of the parameters that take part, which ones: a bit each, or None for all that come);
+        # (None, None) where only the device knows
+        self._host_steps = {}
         self._plans = {}            # group number -> the table of the last step()
         self._captured = []         # tables (and what they point to) that captured graphs read
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -386,8 +388,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"a parameter cannot have {step} steps behind it")
         for gi in range(len(self.param_groups)):
             self._group_steps(gi).fill_(int(step))
-            if self._host_steps.get(gi, 0) is not None:
-                self._host_steps[gi] = int(step)
+            if self._host_steps.get(gi, (0,))[0] is not None:
+                self._host_steps[gi] = (int(step), None)
 
     def state_dict(self):
         """torch's layout; every parameter's state has `step` as a whole number (read from the device)."""
@@ -418,8 +420,11 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p] = {k: st[k].to(p.device, torch.float32 if self.state_bits == 32 else st[k].dtype,
                                                  copy=True) for k in keys}
             self._group_steps(gi).copy_(torch.tensor(steps))
-            if self._host_steps.get(gi, 0) is not None:
-                self._host_steps[gi] = steps[0] if len(set(steps)) == 1 else None
+            if self._host_steps.get(gi, (0,))[0] is not None:
+                taken, mask = set(steps) - {0}, 0
+                for t in steps:
+                    mask = mask << 1 | (t > 0)
+                self._host_steps[gi] = (0, None) if not taken else (taken.pop(), mask) if len(taken) == 1 else (None, None)
 
     # ------------------------------------------------------------------------------------------ step
     def _table(self, gi, group, key, grads):
@@ -483,12 +488,13 @@ class AdamW(torch.optim.Optimizer):
         scales = self.state_bits == 8
         for gi, group in enumerate(self.param_groups):
             # what the table was made of: addresses, sizes, types and layouts
-            key, grads, bits = [group["weight_decay"]], [], 0
+            key, grads, bits, mask = [group["weight_decay"]], [], 0, 0
             for p in group["params"]:
                 g = p.grad
+                mask <<= 1
                 if g is None:
-                    self._host_steps[gi] = None
                     continue
+                mask |= 1
                 st = self.state[p]
                 if not st:
                     self._init_state(p)
@@ -499,7 +505,7 @@ class AdamW(torch.optim.Optimizer):
                         st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
                 if scales:
                     key += (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr())
-            if not grads:
+            if not grads:           # (nobody takes a step: nothing to count)
                 continue
             plan = self._plans.get(gi)
             moved = plan is not None and plan["key"] == key and plan["grads"] != grads
@@ -514,16 +520,19 @@ class AdamW(torch.optim.Optimizer):
             if moved:       # gradients in new storage (a graph's table is its own, and stays)
                 _call(plan["index"], "sca_adamw_set_grads", plan["entries"], plan["n"], (ctypes.c_void_p * len(grads))(*grads))
                 plan["grads"] = grads
-            # As long as all parameters have taken every step and no graph takes steps that nobody here sees, the step number
+            # As long as the same parameters take every step and no graph takes steps that nobody here sees, the step number
             # is given; else the device counts.
-            t = self._host_steps.get(gi, 0)
+            t, of = self._host_steps.get(gi, (0, None))
+            if of is not None and of != mask:
+                t = None
             if torch.cuda.is_current_stream_capturing():    # replays read the table and what it points to
                 self._captured.append((plan, [(p, p.grad, dict(self.state[p])) for p in group["params"]]))
                 plan["captured"] = True
                 if moved:   # the table changes when the graph runs, not now
                     del self._plans[gi]
                 t = None
-            t = self._host_steps[gi] = None if t is None else t + 1
+            t = None if t is None else t + 1
+            self._host_steps[gi] = (t, None if t is None else mask)
             b1, b2 = group["betas"]
             _call(plan["index"], "sca_adamw_step", plan["entries"], plan["n"], plan["chunks"], plan["n_chunks"],
                   self.state_bits, None, t or 0, group["lr"], b1, b2, group["eps"], self.seed, plan["scratch"])

@@ -108,7 +108,7 @@ def test_adamw_steps_known_and_counted(ops, bits):
     """The step number given by the host and the one that the device counts, before and after a parameter misses a step."""
     a, b = params(3), params(3)
     oa, ob = ops.AdamW(a, state_bits=bits), ops.AdamW(b, state_bits=bits)
-    ob._host_steps[0] = None
+    ob._host_steps[0] = (None, None)
     for s in range(6):
         set_grads(a, s)
         set_grads(b, s)
@@ -125,6 +125,38 @@ def test_adamw_steps_known_and_counted(ops, bits):
     set_grads(a, 9)
     oa.step()
     assert [oa.state_dict()["state"][i]["step"] for i in range(4)] == [11] * 4
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_frozen_parameters(ops, bits):
+    """Parameters without gradients take no step and count none; one that joins later starts at its own first step, also after
+    the states went through a state dict."""
+    a, b, c = params(6), params(6), params(6)
+    oa, ob = ops.AdamW(a, state_bits=bits), ops.AdamW(b, state_bits=bits)
+    ob._host_steps[0] = (None, None)                       # counted on the device throughout
+    for s in range(4):
+        for ps in (a, b):
+            set_grads(ps, s)
+            ps[2].grad = None
+        oa.step()
+        ob.step()
+    assert oa._host_steps[0] == (4, 0b1101) and torch.equal(a[2], c[2])
+    oc = ops.AdamW(c, state_bits=bits)
+    oc.load_state_dict(oa.state_dict())
+    for p, q in zip(c, a):
+        p.data.copy_(q.data)
+    assert oc._host_steps[0] == (4, 0b1101)
+    for s in range(4, 8):
+        for ps, o in ((a, oa), (b, ob), (c, oc)):
+            set_grads(ps, s)
+            if s < 6:
+                ps[2].grad = None
+            o.step()
+    for o in (oa, ob, oc):
+        assert [o.state_dict()["state"][i]["step"] for i in range(4)] == [8, 8, 2, 8]
+    for p, q, r in zip(a, b, c):
+        assert torch.equal(p, r)
+        within(p.detach(), q.detach().double(), 64 * U * (q.detach().double().abs() + 1e-2), "p")
 
 
 def test_adamw_first_step_is_not_captured(ops):
