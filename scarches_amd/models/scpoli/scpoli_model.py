@@ -126,7 +126,7 @@ class scPoli(BaseMixin):
               alpha_epoch_anneal=1e2, reload_best: bool = False, prototype_training: Optional[bool] = True,
               unlabeled_prototype_training: Optional[bool] = True, **kwargs):
         """Train with `scPoliTrainer`: `pretraining_epochs` (default 90 % of n_epochs) without, the rest with the
-        prototype loss weighted by `eta`."""
+        prototype loss weighted by `eta`; kwargs are the trainer's (optimizer="adam" or "adamw", ...)."""
         self.prototype_training_ = prototype_training
         self.unlabeled_prototype_training_ = unlabeled_prototype_training
         if self.cell_type_keys_ is None:

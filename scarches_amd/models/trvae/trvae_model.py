@@ -43,7 +43,8 @@ class TRVAE(BaseMixin, SurgeryMixin, CVAELatentsMixin):
         self.trainer = None
 
     def train(self, n_epochs: int = 400, lr: float = 1e-3, eps: float = 0.01, **kwargs):
-        """Train with `trVAETrainer`; kwargs are the trainer's (batch_size, alpha_epoch_anneal, weight_decay, ...)."""
+        """Train with `trVAETrainer`; kwargs are the trainer's (batch_size, alpha_epoch_anneal, weight_decay, optimizer="adam"
+        or "adamw", ...)."""
         self.trainer = trVAETrainer(self.model, self.adata, condition_key=self.condition_key_, **kwargs)
         self.trainer.train(n_epochs, lr, eps)
         self.is_trained_ = True

@@ -179,3 +179,43 @@ def test_csr_rows_in_8_bit_integers(G, nnz, log1p):
                                              q.data_ptr(), pitch, s.data_ptr(), st), "csr_quant_rows_i8")
         assert torch.equal(q[:B, :G], want) and torch.equal(s.view(torch.int32), scale.view(torch.int32))
         assert not q[:B, G:].any() and (q[B] == 77).all()               # padded with zeros; the row behind is left alone
+
+
+def small_model(model):
+    from scarches_amd.anndata_lite import CellData
+    from scarches_amd.models import EXPIMAP, TRVAE, scPoli
+    X, obs = synth(400, 64, 3, 3, seed=5)
+    ad = CellData(X, obs)
+    torch.manual_seed(0)
+    if model == "trvae":
+        return TRVAE(ad, condition_key="study", hidden_layer_sizes=[32], latent_dim=5)
+    if model == "expimap":
+        mask = np.random.default_rng(2).random((8, 64)) < 0.4             # [programs, genes]
+        return EXPIMAP(ad, condition_key="study", hidden_layer_sizes=[32, 32], mask=mask.astype(np.float32), recon_loss="nb")
+    return scPoli(ad, condition_keys="study", cell_type_keys="cell_type", hidden_layer_sizes=[32], latent_dim=5, embedding_dims=3)
+
+
+def test_expimap_trains_with_adamw():
+    with contextlib.redirect_stdout(io.StringIO()):
+        m = small_model("expimap")
+        start = {k: v.clone() for k, v in m.model.state_dict().items()}
+        m.train(n_epochs=2, lr=1e-3, batch_size=64, monitor=False, optimizer="adamw", weight_decay=10.0, alpha=1e-4)
+    eng = m.model.engine()
+    assert eng.optimizer == "adamw"
+    name = next(k for k in start if k.startswith("encoder") and k.endswith("expr_L.weight"))
+    now, was = m.model.state_dict()[name].cpu(), start[name].cpu()
+    assert eng.adam_t > 0 and (now - was).abs().max() <= eng.adam_t * 1e-3 * (10 * was.abs().max() + 4)
+    assert torch.isfinite(now).all() and not torch.equal(now, was)
+
+
+@pytest.mark.parametrize("model", ["trvae", "expimap", "scpoli"])
+def test_latent_from_csr_and_from_dense_rows(model, monkeypatch):
+    """get_latent(int8=True) gives the same bits whether the cells go to 8-bit integers from CSR or from gathered rows."""
+    with contextlib.redirect_stdout(io.StringIO()):
+        m = small_model(model)
+        args = (m.adata.X, m.adata.obs["study"]) if model != "scpoli" else (m.adata,)
+        one = m.get_latent(*args, mean=True, int8=True)
+        monkeypatch.setattr(type(m.model.engine()), "_quantized_cells", lambda *a: None)
+        two = m.get_latent(*args, mean=True, int8=True)
+        exact = m.get_latent(*args, mean=True)
+    assert np.array_equal(one, two) and np.isfinite(one).all() and not np.array_equal(one, exact)
