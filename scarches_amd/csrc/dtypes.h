@@ -37,6 +37,27 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[N]
     for (int i = 0; i < N; ++i) t[i] = from_f32<T>(v[i]);
     __builtin_memcpy(p, t, sizeof(T) * N);
 }
+// The same past the caches, for results that are larger than they are (what reads them next would not find them there).
+typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
+template <typename T, int N>
+__device__ __forceinline__ void stream_vec(T* __restrict__ p, const float (&v)[N]) {
+    typedef words4 words4_at __attribute__((aligned(2)));
+    typedef words2 words2_at __attribute__((aligned(2)));
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = from_f32<T>(v[i]);
+    static_assert(sizeof(T) * N == 16 || sizeof(T) * N == 8, "one store");
+    if constexpr (sizeof(T) * N == 16) {
+        words4 w;
+        __builtin_memcpy(&w, t, 16);
+        __builtin_nontemporal_store(w, (words4_at*)p);
+    } else {
+        words2 w;
+        __builtin_memcpy(&w, t, 8);
+        __builtin_nontemporal_store(w, (words2_at*)p);
+    }
+}
 // The first `left` of N elements (the others read as 0 / are not written).
 template <typename T, int N>
 __device__ __forceinline__ void load_part(const T* __restrict__ p, int left, float (&v)[N]) {

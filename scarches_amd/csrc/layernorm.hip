@@ -35,7 +35,7 @@ template <typename T, typename W, int TPR, int V, int MODE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_kernel(const T* __restrict__ x, long long ldx,
                                                                        long long rows, int n, const W* __restrict__ w,
                                                                        const W* __restrict__ b, float eps,
-                                                                       T* __restrict__ y, long long ldy,
+                                                                       T* __restrict__ y, long long ldy, bool stream,
                                                                        float* __restrict__ stats) {
     constexpr int VEC = vec_of<T>(), NT = TPR > 256 ? TPR : 256;
     __shared__ float scratch[16];
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_kernel(const T* 
             unpack_again<T>(raw[j], v);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, g[i], o[i]);
-            store_cols<MODE>(yr, at.c, n, v);
+            store_cols<MODE>(yr, at.c, n, v, stream);
         }
         if (t == 0 && stats) {
             stats[r] = mean;
@@ -97,7 +97,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_kernel(const T* 
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, long long ldx, long long rows, int n,
                                                            const W* __restrict__ w, const W* __restrict__ b, float eps,
-                                                           T* __restrict__ y, long long ldy, float* __restrict__ stats) {
+                                                           T* __restrict__ y, long long ldy, bool stream,
+                                                           float* __restrict__ stats) {
     constexpr int VEC = vec_of<T>();
     __shared__ float scratch[16];
     const int vecs = (n + VEC - 1) / VEC;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
             load_vec<T, VEC>(xr + col(j), v);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, g[i], o[i]);
-            store_vec<T, VEC>(y + r * ldy + col(j), v);
+            store_cols<ROW_RAGGED>(y + r * ldy, col(j), n, v, stream);
         }
         if (threadIdx.x == 0 && stats) {
             stats[r] = mean;
@@ -146,7 +147,7 @@ struct LnBwd {
     long long rows; int n;
     const void* w;
     const float* stats;
-    void* dx; long long lddx;
+    void* dx; long long lddx; bool stream;
     float* part;                 // [slab][2][n] partial sums of (dw, db), or null
     float* means;                // rows beyond the registers: [2][rows]
 };
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
             unpack_again<T>(d0[j], d);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) d[i] = rstd0 * (fmaf(d[i], g[j][i], -m1) - (h[i] - mean0) * rstd0 * m2);
-            store_cols<MODE>(out, at.c, n, d);
+            store_cols<MODE>(out, at.c, n, d, a.stream);
         }
     }
     if (!a.part) return;
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(256) void ln_bwd_long_kernel(const LnBwd a) {
             const float m1 = a.means[r + u], m2 = a.means[a.rows + r + u];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) d[i] = rstd * (fmaf(d[i], g[i], -m1) - h[i] * m2);
-            store_vec<T, VEC>((T*)a.dx + (r + u) * a.lddx + c, d);
+            store_cols<ROW_RAGGED>((T*)a.dx + (r + u) * a.lddx, c, n, d, a.stream);
         }
     }
     if (!a.part) return;
@@ -365,6 +366,12 @@ __global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restr
 constexpr int CUS = 256;
 constexpr int MAX_HELD = 16384;                   // longest row of the backward pass in registers
 
+// Results of 100 MB and more are stored past the caches (us without / with, GPU busy with this alone: forward of 16384 x
+// 4000 fp32 97 / 77, bf16 44.4 / 43.1, and 59 / 53 on inputs that are in no cache; backward of the bf16 rows 82 / 68).  Of
+// less, the caches keep a part for the operator that reads them next, and 8192 x 2000 fp32 (66 MB) gains nothing: 22.2 / 21.5
+// and 35.7 / 37.7.
+bool past_the_caches(long long rows, int n, size_t size) { return (double)rows * n * size >= 1e8; }
+
 // How the backward pass holds a row of `vecs` vectors: TPR threads, at most 32 elements each (five values are kept per
 // element); 0: not at all.  nt: threads of a workgroup - half as many where there are not enough rows to give every CU
 // eight waves.  Four waves a row and four rows a workgroup (us of one wave a row / this; 1000, 2000, 8000 rows): fp32 of 493
@@ -397,9 +404,10 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
            long long ldy, float* stats, hipStream_t st) {
     constexpr int VEC = vec_of<T>();
     const int vecs = (n + VEC - 1) / VEC, mode = row_mode(n, VEC);
+    const bool stream = past_the_caches(rows, n, sizeof(T));
 #define FWD_MODE(TPR, V, MODE)                                                                                           \
     hipLaunchKernelGGL((ln_fwd_kernel<T, W, TPR, V, MODE>), dim3((unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS)), \
-                       dim3(NT), 0, st, (const T*)x, ldx, rows, n, (const W*)w, (const W*)b, eps, (T*)y, ldy, stats)
+                       dim3(NT), 0, st, (const T*)x, ldx, rows, n, (const W*)w, (const W*)b, eps, (T*)y, ldy, stream, stats)
 #define FWD(TPR, V)                                                             \
     do {                                                                        \
         constexpr int NT = TPR > 256 ? TPR : 256;                               \
@@ -428,7 +436,7 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
     else if (vecs <= 4096) FWD(1024, 4);
     else
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(1024), 0, st, (const T*)x, ldx, rows, n,
-                           (const W*)w, (const W*)b, eps, (T*)y, ldy, stats);
+                           (const W*)w, (const W*)b, eps, (T*)y, ldy, stream, stats);
 #undef FWD
 #undef FWD_MODE
     SCA_CHECK_LAUNCH();
@@ -440,6 +448,7 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
     constexpr int VEC = vec_of<T>(), V = 32 / VEC;
     const int n = a.n, vecs = (n + VEC - 1) / VEC, mode = row_mode(n, VEC);
     const BwdShape sh = bwd_shape(a.rows, n, VEC);
+    a.stream = past_the_caches(a.rows, n, sizeof(T));
     if (a.rows > 0 && sh.tpr) {
 #define BWD_MODE(TPR, V, MODE, NT)                                                                                        \
     hipLaunchKernelGGL((ln_bwd_kernel<T, W, TPR, V, MODE, NT>), dim3((unsigned)sh.slabs), dim3(NT), 0, st, a)
@@ -517,7 +526,7 @@ extern "C" int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, 
     if (rows > 0 && (!dy || !x || !stats)) return -1;
     if (!dx && !dw && !db) return 0;
     if (!ws && (dw || db || n > MAX_HELD)) return -1;
-    LnBwd a{dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, dw || db ? ws : nullptr, nullptr};
+    LnBwd a{dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, false, dw || db ? ws : nullptr, nullptr};
     if (n > MAX_HELD) a.means = ws + 2LL * n * bwd_shape(rows, n, dtype == SCA_F32 ? 4 : 8).slabs;
     return LN_DISPATCH(ln_bwd, a, dw, db, (hipStream_t)stream);
 }

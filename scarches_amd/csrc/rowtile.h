@@ -81,8 +81,9 @@ __device__ __forceinline__ void unpack_again(raw_t& raw, float (&v)[vec_of<T>()]
     unpack<T>(raw, v);
 }
 template <int MODE, typename T, int VEC>
-__device__ __forceinline__ void store_cols(T* __restrict__ row, int c, int n, const float (&v)[VEC]) {
+__device__ __forceinline__ void store_cols(T* __restrict__ row, int c, int n, const float (&v)[VEC], bool stream) {
     if (MODE == ROW_TINY) store_part<T, VEC>(row, n, v);
+    else if (stream) stream_vec<T, VEC>(row + c, v);
     else store_vec<T, VEC>(row + c, v);
 }
 
