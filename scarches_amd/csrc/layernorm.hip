@@ -434,6 +434,8 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
     else if (vecs <= 1024) FWD(256, 4);
     else if (vecs <= 2048) FWD(1024, 2);
     else if (vecs <= 4096) FWD(1024, 4);
+    else if (vecs <= 5120) FWD(1024, 5);
+    else if (VEC == 4 && vecs <= 8192) FWD(1024, (VEC == 4 ? 8 : 5));
     else
         hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(1024), 0, st, (const T*)x, ldx, rows, n,
                            (const W*)w, (const W*)b, eps, (T*)y, ldy, stream, stats);
