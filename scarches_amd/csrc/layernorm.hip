@@ -152,22 +152,28 @@ struct LnBwd {
     float* means;                // rows beyond the registers: [2][rows]
 };
 
-// NT threads, TPR of them a row.
-template <typename T, typename W, int TPR, int V, int MODE, int NT>
+// NT threads, TPR of them a row.  HOLD: the weight stays in registers; the longest rows read it again (from a cache).
+template <typename T, typename W, int TPR, int V, int MODE, int NT, bool HOLD = true>
 __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
     constexpr int VEC = vec_of<T>(), PER = NT / TPR, COLS = TPR * V * VEC;
     __shared__ float scratch[16];
     __shared__ __attribute__((aligned(16))) float sums[PER > 1 ? PER * COLS : 4];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, n = a.n;
     const float inv_n = 1.f / (float)n;
-    float g[V][VEC], dw[V][VEC], db[V][VEC];
+    float held[HOLD ? V : 1][VEC], dw[V][VEC], db[V][VEC];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const Cols<T, TPR, MODE> at(j, t, n);
-        if (at.there) load_weight<MODE>((const W*)a.w, at.c, n, 1.f, g[j]);
+        if (HOLD && at.there) load_weight<MODE>((const W*)a.w, at.c, n, 1.f, held[HOLD ? j : 0]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dw[j][i] = db[j][i] = 0.f;
     }
+    auto weight = [&](int j, int c, float (&g)[VEC]) {
+        if (!HOLD) load_weight<MODE>((const W*)a.w, c, n, 1.f, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (HOLD) g[i] = held[HOLD ? j : 0][i];
+    };
     const long long step = (long long)gridDim.x * PER;
     raw_t xq[V] = {}, dq[V] = {};
     float mean = 0.f, rstd = 0.f;
@@ -186,7 +192,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
     };
     // 16-bit rows, whose arithmetic takes half as long as their loads: the next row is on its way meanwhile (16384 x 4000
     // bf16: 81 instead of 100 us).  fp32 rows have no registers for it and run at the rate of a copy without.
-    constexpr bool AHEAD = sizeof(T) == 2;
+    constexpr bool AHEAD = sizeof(T) == 2 && HOLD;
     // (where rows meet at barriers, a wave without a row of its own goes along with zeros)
     constexpr bool TOGETHER = PER > 1 && TPR > 64;
     long long r = (long long)blockIdx.x * PER + sub;
@@ -202,11 +208,12 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
             d0[j] = mine ? dq[j] : raw_t{0, 0, 0, 0};
         }
         if (AHEAD && r + step < a.rows) load(r + step);
-        float s1 = 0.f, s2 = 0.f, h[VEC], d[VEC];
+        float s1 = 0.f, s2 = 0.f, h[VEC], d[VEC], g[VEC];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const Cols<T, TPR, MODE> at(j, t, n);
             if (!at.there) continue;
+            weight(j, at.c, g);
             unpack<T>(x0[j], h);
             unpack<T>(d0[j], d);
 #pragma unroll
@@ -214,7 +221,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
                 h[i] = (h[i] - mean0) * rstd0;
                 dw[j][i] = fmaf(d[i], h[i], dw[j][i]);
                 db[j][i] += d[i];
-                const float p = at.own(i, n) ? d[i] * g[j][i] : 0.f;
+                const float p = at.own(i, n) ? d[i] * g[i] : 0.f;
                 s1 += p;
                 s2 = fmaf(p, h[i], s2);
             }
@@ -226,10 +233,11 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
         for (int j = 0; j < V; ++j) {
             const Cols<T, TPR, MODE> at(j, t, n);
             if (!at.there || !mine) continue;
+            weight(j, at.c, g);
             unpack_again<T>(x0[j], h);
             unpack_again<T>(d0[j], d);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) d[i] = rstd0 * (fmaf(d[i], g[j][i], -m1) - (h[i] - mean0) * rstd0 * m2);
+            for (int i = 0; i < VEC; ++i) d[i] = rstd0 * (fmaf(d[i], g[i], -m1) - (h[i] - mean0) * rstd0 * m2);
             store_cols<MODE>(out, at.c, n, d, a.stream);
         }
     }
@@ -262,7 +270,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
     put(db, slab + n);
 }
 
-// Rows beyond the registers (20000 and more genes).  Both operands are read twice: once row by row for the two means, one
+// Rows beyond the registers.  Both operands are read twice: once row by row for the two means, one
 // workgroup per row, and once by columns, for dx and the sums of dw and db together.  (500 x 40000 fp32:
 // 71 us, 3.4 TB/s by the three arrays.)
 template <typename T, typename W>
@@ -364,7 +372,10 @@ __global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restr
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 constexpr int CUS = 256;
-constexpr int MAX_HELD = 16384;                   // longest row of the backward pass in registers
+// Longest row of the backward pass in registers: four (fp32) or two (16 bits) vectors of 1024 threads, and one more where
+// there are rows enough that the partial sums, two rows of every workgroup, weigh little (us of reading twice / this, fp32
+// rows of 20000: 64 rows 14.6 / 17.1, 1000 68 / 66, 4000 284 / 211).
+constexpr int max_held(int vec, long long rows) { return rows < 512 ? 16384 : vec == 4 ? 20480 : 24576; }
 
 // Results of 100 MB and more are stored past the caches (us without / with, GPU busy with this alone: forward of 16384 x
 // 4000 fp32 97 / 77, bf16 44.4 / 43.1, and 59 / 53 on inputs that are in no cache; backward of the bf16 rows 82 / 68).  Of
@@ -385,7 +396,7 @@ BwdShape bwd_shape(long long rows, int n, int vec) {
     const int vecs = (n + vec - 1) / vec, v = 32 / vec;
     BwdShape s;
     const bool four = vecs > 128 && vecs <= 512 && (vecs > 256 || rows <= 8 * CUS);
-    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 && !four ? 64 : vecs <= 256 * v ? 256 : n <= MAX_HELD ? 1024 : 0;
+    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 && !four ? 64 : vecs <= 256 * v ? 256 : n <= max_held(vec, rows) ? 1024 : 0;
     s.nt = four ? 1024 : s.tpr > 64 ? s.tpr : rows * s.tpr <= 512 * CUS ? 256 : 512;
     if (s.tpr == 0) {
         const long long wide = (n + 256LL * vec - 1) / (256LL * vec), want = 4 * CUS / wide, most = (rows + 7) / 8;
@@ -452,8 +463,8 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
     const BwdShape sh = bwd_shape(a.rows, n, VEC);
     a.stream = past_the_caches(a.rows, n, sizeof(T));
     if (a.rows > 0 && sh.tpr) {
-#define BWD_MODE(TPR, V, MODE, NT)                                                                                        \
-    hipLaunchKernelGGL((ln_bwd_kernel<T, W, TPR, V, MODE, NT>), dim3((unsigned)sh.slabs), dim3(NT), 0, st, a)
+#define BWD_MODE(TPR, V, MODE, ...)                                                                                       \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, W, TPR, V, MODE, __VA_ARGS__>), dim3((unsigned)sh.slabs), dim3(sh.nt), 0, st, a)
 #define BWD(TPR, V, NT)                                         \
     do {                                                        \
         if (mode == ROW_FULL) BWD_MODE(TPR, V, ROW_FULL, NT);   \
@@ -475,7 +486,9 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
         else if (vecs <= 64 * 2) BWD2(64, 2);
         else if (vecs <= 64 * 4) BWD2(64, 4);
         else if (vecs <= 256 * V) BWD(256, V, 256);
-        else BWD(1024, V / 2, 1024);
+        else if (vecs <= 1024 * (V / 2)) BWD(1024, V / 2, 1024);
+        else if (mode == ROW_FULL) BWD_MODE(1024, V / 2 + 1, ROW_FULL, 1024, false);
+        else BWD_MODE(1024, V / 2 + 1, ROW_RAGGED, 1024, false);
 #undef BWD2
 #undef BWD
 #undef BWD_MODE
@@ -527,8 +540,9 @@ extern "C" int sca_layernorm_bwd(const void* dy, long long lddy, const void* x, 
     if (!ln_types_ok(dtype, wtype) || rows < 0 || n <= 0 || n > MAX_N || lddy < 0 || ldx < 0 || (dx && lddx < n)) return -1;
     if (rows > 0 && (!dy || !x || !stats)) return -1;
     if (!dx && !dw && !db) return 0;
-    if (!ws && (dw || db || n > MAX_HELD)) return -1;
+    const int vec = dtype == SCA_F32 ? 4 : 8;
+    if (!ws && (dw || db || n > max_held(vec, rows))) return -1;
     LnBwd a{dy, lddy, x, ldx, rows, n, w, stats, dx, lddx, false, dw || db ? ws : nullptr, nullptr};
-    if (n > MAX_HELD) a.means = ws + 2LL * n * bwd_shape(rows, n, dtype == SCA_F32 ? 4 : 8).slabs;
+    if (n > max_held(vec, rows)) a.means = ws + 2LL * n * bwd_shape(rows, n, vec).slabs;
     return LN_DISPATCH(ln_bwd, a, dw, db, (hipStream_t)stream);
 }

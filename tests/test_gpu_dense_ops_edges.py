@@ -20,7 +20,7 @@ def ops():
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("layout", ["plain", "odd", "expanded"])
-@pytest.mark.parametrize("rows,n", [(1, 16385), (7, 33538), (600, 20001), (9, 131072)])
+@pytest.mark.parametrize("rows,n", [(1, 16385), (7, 33538), (600, 20001), (9, 131072), (300, 20480), (520, 20477), (700, 24573), (40, 40960)])
 def test_layer_norm_long_rows(ops, rows, n, layout, dtype):
     x, dy = matrix(rows, n, dtype, n, layout), matrix(rows, n, dtype, n + 1, layout)
     w = (1 + 0.2 * torch.randn(n, device="cuda", generator=gen(1))).to(dtype)

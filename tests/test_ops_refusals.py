@@ -133,7 +133,7 @@ def test_too_wide():
     assert lib.sca_quant_rows_i8(a, n, 0, 1, n, a, n, a, None) == -1
     assert lib.sca_gemm_i8(a, 4, a, a, 4, a, None, 0, 1, n, 4, a, 0, n, None) == -1
     # rows beyond the registers need the workspace for dx as well
-    assert lib.sca_layernorm_bwd(a, 16385, a, 16385, 0, 1, 16385, None, 0, a, a, 16385, None, None, None, None) == -1
+    assert lib.sca_layernorm_bwd(a, 30000, a, 30000, 0, 1, 30000, None, 0, a, a, 30000, None, None, None, None) == -1
     assert lib.sca_adamw_set_grads(None, 1, a, None) == -1 and lib.sca_adamw_set_grads(a, -1, a, None) == -1
     assert lib.sca_adamw_set_grads(None, 0, None, None) == 0
     with pytest.raises(ValueError):
