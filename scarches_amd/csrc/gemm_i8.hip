@@ -738,6 +738,8 @@ void quant_rows(const void* x, long long ldx, long long rows, int k, int8_t* q, 
     if (vecs <= 1024) QUANT(256, 4);
     if (vecs <= 2048) QUANT(1024, 2);
     if (vecs <= 4096) QUANT(1024, 4);
+    if (vecs <= 5120) QUANT(1024, 5);
+    if (vecs <= 8192) QUANT(1024, 8);
 #undef QUANT
     hipLaunchKernelGGL((quant_rows_long_kernel<T>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(1024), 0,
                        st, (const T*)x, ldx, rows, k, q, ldq, scale);

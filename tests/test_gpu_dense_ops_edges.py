@@ -4,10 +4,11 @@ at every step, calls side by side on two streams.  Bounds as in test_gpu_dense_o
 import copy
 import io
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_dense_ops import TYPES, U, gen, ln_check_bwd, ln_check_fwd, matrix, within
+from tests.test_gpu_dense_ops import TYPES, U, gen, ln_check_bwd, ln_check_fwd, matrix, quant_ref, within
 
 pytestmark = pytest.mark.gpu
 
@@ -256,3 +257,50 @@ def test_two_streams(ops):
         for one, two in zip(alone, together):
             for a, b in zip(one, two):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,k", [(5, 16388), (3, 20480), (4, 20481), (3, 32768), (2, 32771), (3, 40960), (2, 40961), (2, 65536), (2, 65537)])
+def test_quantize_long_rows(ops, rows, k, dtype):
+    x = matrix(rows, k, dtype, rows + k, "odd", scale=3.0)
+    q, s = ops.quantize_int8(x)
+    rq, rs = quant_ref(x.float().cpu().numpy())
+    assert torch.equal(s.cpu(), torch.from_numpy(rs)) and torch.equal(q.cpu(), torch.from_numpy(rq))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("power", [0, -9, 7])
+def test_quantize_every_short_value(ops, dtype, power):
+    """Rows that hold every value of the type in the nine binades below their largest, for every fraction of the largest (bf16;
+    every ninth of fp16): the quotients lie next to the middles between two integers all the time."""
+    bits = 7 if dtype == torch.bfloat16 else 10
+    frac = torch.arange(2 ** bits, 2 ** (bits + 1), dtype=torch.float64) / 2 ** bits          # [1, 2)
+    values = torch.cat([frac * 2.0 ** -e for e in range(9)])
+    values = torch.cat([values, -values])
+    top = frac if bits == 7 else frac[::9]
+    x = torch.where(values.abs()[None] <= top[:, None], values[None], torch.zeros(()).double())
+    x = torch.cat([x, top[:, None]], 1) * 2.0 ** power
+    x = x.to(dtype)                     # (exact but for what fp16 holds as denormal numbers, below 2^-14)
+    q, s = ops.quantize_int8(x.cuda())
+    rq, rs = quant_ref(x.float().numpy())
+    assert torch.equal(s.cpu(), torch.from_numpy(rs)) and torch.equal(q.cpu(), torch.from_numpy(rq))
+
+
+def test_quantize_next_to_every_middle(ops):
+    """fp32 rows of random scales with the values next to all 127 middles, up to three steps of the type to either side."""
+    g = np.random.default_rng(3)
+    top = (g.random(400) + 0.5).astype(np.float32) * np.exp2(g.integers(-60, 60, 400)).astype(np.float32)
+    top[:3] = 127.0, 254.0, 1.0
+    s = top / np.float32(127)
+    mid = np.float32((np.arange(127) + 0.5) * s.astype(np.float64)[:, None])
+    rows = [top[:, None]]
+    for direction in (np.float32(0), np.float32(np.inf)):
+        v = mid
+        for _ in range(4):
+            rows += [v, -v]
+            v = np.nextafter(v, direction)
+    x = np.minimum(np.maximum(np.concatenate(rows, 1), -top[:, None]), top[:, None]).astype(np.float32)
+    q, sc = ops.quantize_int8(torch.from_numpy(x).cuda())
+    rq, rs = quant_ref(x)
+    np.testing.assert_array_equal(sc.cpu().numpy(), rs)
+    np.testing.assert_array_equal(q.cpu().numpy(), rq)
