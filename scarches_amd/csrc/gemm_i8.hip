@@ -220,11 +220,21 @@ __global__ __launch_bounds__(64) void csr_quant_rows_kernel(const int64_t* __res
     if (threadIdx.x == 0) scale[b] = sc.s;
 }
 
-__device__ __forceinline__ i32x4 load16(const int8_t* p, int left) {
+// 16 bytes at p, of which `left` belong to the row of K bytes (what lies behind counts as 0).  The row's end is read as the 16
+// bytes that end with it, moved down: a byte at a time takes sixteen loads (a row shorter than that has no other way).
+__device__ __forceinline__ i32x4 load16(const int8_t* p, int left, int K) {
     i32x4 v = {0, 0, 0, 0};
     if (left >= 16) {
         __builtin_memcpy(&v, p, 16);
-    } else {
+    } else if (left > 0 && K >= 16) {
+        uint64_t w[2];
+        __builtin_memcpy(w, p - (16 - left), 16);
+        const int shift = 8 * (16 - left);
+        const uint64_t lo = shift < 64 ? w[0] >> shift | w[1] << 1 << (63 - shift) : w[1] >> (shift - 64);
+        w[1] = shift < 64 ? w[1] >> shift : 0;
+        w[0] = lo;
+        __builtin_memcpy(&v, w, 16);
+    } else if (left > 0) {
         int8_t b[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) b[i] = i < left ? p[i] : 0;
@@ -298,7 +308,7 @@ __global__ __launch_bounds__(512) void gemm_i8_direct_kernel(const I8Args a) {
             for (int u = 0; u < U; ++u) __builtin_memcpy(&v[u], p + k0 + u * 64, 16);
         } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load16(p + k0 + u * 64, a.K - k0 - u * 64 - ko);
+            for (int u = 0; u < U; ++u) v[u] = load16(p + k0 + u * 64, a.K - k0 - u * 64 - ko, a.K);
         }
     };
     const int k_first = wave * 64 * U;
@@ -410,7 +420,7 @@ __device__ __forceinline__ void stage_load(const int8_t* __restrict__ p, long lo
         const int slot = i * NT + t;
         const int r = slot / C, c = (slot % C) ^ swap_of<KB>(r);
         const long long row = r0 + r < rows ? r0 + r : rows - 1;
-        v[i] = load16(p + row * ld + k0 + c * 16, K - k0 - c * 16);
+        v[i] = load16(p + row * ld + k0 + c * 16, K - k0 - c * 16, K);
     }
 }
 template <int ROWS, int KB, int NT>
