@@ -304,3 +304,19 @@ def test_quantize_next_to_every_middle(ops):
     rq, rs = quant_ref(x)
     np.testing.assert_array_equal(sc.cpu().numpy(), rs)
     np.testing.assert_array_equal(q.cpu().numpy(), rq)
+
+
+@pytest.mark.parametrize("m,n,ks", [(33, 40, range(1, 300)), (2000, 512, range(391, 660, 11)), (4096, 800, range(123, 400, 13)),
+                                    (8192, 1536, range(60, 330, 27))])
+def test_int8_every_tail(ops, m, n, ks):
+    """Rows of every length: small integers, whose products' sums fp32 holds exactly, with padded and with packed rows."""
+    g = gen(m)
+    for k in ks:
+        pitch = -(-k // 128) * 128
+        xq, wq = (torch.full((s, pitch), 100, dtype=torch.int8, device="cuda")[:, :k] for s in (m, n))
+        xq.random_(-3, 4, generator=g)
+        wq.random_(-3, 4, generator=g)
+        want = (xq.float() @ wq.float().t().contiguous())
+        one_m, one_n = torch.ones(m, device="cuda"), torch.ones(n, device="cuda")
+        for x, w in ((xq, wq), (xq.contiguous(), wq.contiguous())):
+            assert torch.equal(ops.int8_matmul(x, one_m, w, one_n), want), (k, x.stride())
