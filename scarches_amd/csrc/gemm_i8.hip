@@ -271,7 +271,7 @@ __device__ __forceinline__ float bias_at(const I8Args& a, int n) {
 // No staging, no barrier in the k loop: every wave has its whole share of both operands in flight.
 // T = int8_t: x is quantized.  Else every workgroup quantizes the (at most QUANT_ROWS) rows itself, into LDS, while its
 // weights are on their way: for single rows a launch of its own costs more than this repeated work (1 x 4096 x 4000:
-// 6.4 us instead of 2.7 + 5.4; at four rows 11.2 instead of 9.2).
+// 5.9 us instead of 2.9 + 4.9; four rows took 11.2 instead of 9.2).
 constexpr int QUANT_ROWS = 2, QUANT_K = 8192;
 
 // Columns [c, c + VEC) of a row of n; what lies behind the end reads as 0.
@@ -775,22 +775,28 @@ void launch_direct(I8Args a, hipStream_t st) {
     hipLaunchKernelGGL((gemm_i8_direct_kernel<T>), dim3((unsigned)((long long)a.tiles_m * a.tiles_n)), dim3(512), 0, st, a);
 }
 
-// Which kernel: us of direct / 64 x 64 by four groups / 128 x 128 / 256 x 256 tiles, results in bf16:
-//   1 x 4096 x 4000 (M x N x K)   5.4 / 10.6 / 18 / 44       512 x 512 x 2048     9.9 / 6.4 / 10.6 / 25
-//   128 x 128 x 2000              4.3 / 8.3 / 13 / 27        8192 x 128 x 2000    27 / 9.7 / 13.5 / 28
-//   300 x 300 x 4096              9.8 / 8.7 / 18 / 46        1024 x 1024 x 4096   63 / 10.6 / 20 / 43
-//   2048 x 2048 x 2048            - / 26 / 14.5 / 29         16384 x 256 x 4000   - / 52 / 30 / 51
-//   4096 x 4096 x 4096            - / 156 / 88 / 72          65536 x 64 x 512     - / 17 / 11.7 / 16.6
-// Larger tiles read less; they need about one tile per CU, and little of it lost behind the edges.
+// Which kernel: us of direct / 64 x 64 by four groups / 128 x 128 / 256 x 256 tiles, results in bf16 (M x N x K):
+//   1 x 4096 x 4000     4.9 / 9.2 / 17 / 43           512 x 512 x 2048      10.0 / 6.4 / 10.5 / 25
+//   16 x 8192 x 4000    10.2 / 11.0 / 18 / -          8192 x 128 x 2000     37 / 7.7 / 11.9 / 27
+//   128 x 128 x 2000    4.4 / 6.7 / 11.4 / 26         1024 x 1024 x 4096    59 / 10.3 / 20 / 43
+//   256 x 256 x 8000    9.8 / 14.3 / 27 / -           64 x 20000 x 128      15.5 / 8.7 / 5.3 / -
+//   320 x 400 x 2000    6.4 / 6.9 / 11.5 / -          2048 x 2048 x 2048    118 / 24 / 13.7 / 28
+//   300 x 300 x 4096    9.7 / 8.7 / 18 / 46           16384 x 256 x 4000    224 / 43 / 25 / 46
+//   509 x 282 x 1972    8.3 / 7.5 / 12.6 / 28         4096 x 4096 x 4096    - / 156 / 84 / 69
+//   1000 x 250 x 300    6.1 / 5.4 / 8.1 / -           65536 x 64 x 512      40 / 17 / 10.9 / 16.1
+// Direct: one workgroup per CU at most, or a few with short rows (or single cells, whose x is read from the caches); 64: no
+// more tiles than CUs.  Larger tiles read less; they need about one tile per CU, and little of it lost behind the edges.
+constexpr int CUS = 256;
 void gemm_i8(const I8Args& a, hipStream_t st) {
     const bool aligned = !(((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.ldx | (uintptr_t)a.ldw) & 15);
     auto tiles = [&](int b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
-    const bool fits = ((a.M + 15) / 16) * ((a.N + 15) / 16) < 1 << 23;          // fewer than 2^32 threads
-    if (fits && (a.M <= 16 || (double)a.M * a.N * a.K < 4e8)) {
+    const long long t16 = tiles(16);
+    const bool fits = t16 < 1 << 23;                                            // fewer than 2^32 threads
+    if (fits && (a.M <= 16 || t16 <= CUS || (t16 <= 5 * CUS / 2 && t16 * a.K <= 1 << 20))) {
         launch_direct<int8_t>(a, st);
     } else if (aligned && tiles(256) >= 192 && 16 * tiles(256) <= 5 * tiles(128)) {
         launch_tile<256, 256, 2, 4, 64, 4, 1, true>(a, st);
-    } else if (tiles(128) >= 192) {
+    } else if (tiles(64) > CUS) {
         if (aligned) launch_tile<128, 128, 2, 2, 64, 4, 1, true>(a, st);
         else launch_tile<128, 128, 2, 2, 64, 4, 1, false>(a, st);
     } else {
