@@ -787,12 +787,15 @@ void launch_direct(I8Args a, hipStream_t st) {
 // Direct: one workgroup per CU at most, or a few with short rows (or single cells, whose x is read from the caches); 64: no
 // more tiles than CUs.  Larger tiles read less; they need about one tile per CU, and little of it lost behind the edges.
 constexpr int CUS = 256;
+bool takes_direct(long long M, int N, int K) {
+    const long long tiles = ((M + 15) / 16) * ((N + 15LL) / 16);
+    if (tiles >= 1 << 23) return false;                                         // (fewer than 2^32 threads)
+    return M <= 16 || tiles <= CUS || (tiles <= 5 * CUS / 2 && tiles * K <= 1200000);
+}
 void gemm_i8(const I8Args& a, hipStream_t st) {
     const bool aligned = !(((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.ldx | (uintptr_t)a.ldw) & 15);
     auto tiles = [&](int b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
-    const long long t16 = tiles(16);
-    const bool fits = t16 < 1 << 23;                                            // fewer than 2^32 threads
-    if (fits && (a.M <= 16 || t16 <= CUS || (t16 <= 5 * CUS / 2 && t16 * a.K <= 1 << 20))) {
+    if (takes_direct(a.M, a.N, a.K)) {
         launch_direct<int8_t>(a, st);
     } else if (aligned && tiles(256) >= 192 && 16 * tiles(256) <= 5 * tiles(128)) {
         launch_tile<256, 256, 2, 4, 64, 4, 1, true>(a, st);
@@ -815,7 +818,12 @@ void quantize(const void* x, long long ldx, int dtype, long long rows, int k, in
     else quant_rows<sca_f16>(x, ldx, rows, k, q, ldq, scale, st);
 }
 bool one_launch(long long M, int K) { return M <= QUANT_ROWS && K <= QUANT_K - 128; }
-long long pitch_of(int K) { return ((long long)K + 127) & ~127LL; }
+// Pitch of the rows that sca_linear_i8 quantizes for itself.  Tiles want whole cache lines (128 x 128 tiles, 16384 x 256 x
+// 4000: 25.0 us, 28.8 with 16 bytes more); the direct kernel, whose 16 lanes read 16 rows, wants them to start in different
+// banks (16 x 4096 x 4000: 6.6 us on whole lines, 5.5 with an odd number of 16-byte pieces; 320 x 400 x 2000: 6.4, 5.2).
+long long pitch_of(int K, bool direct) {
+    return direct ? (((long long)K + 15) / 16 | 1) * 16 : ((long long)K + 127) & ~127LL;
+}
 
 }  // namespace
 
@@ -858,7 +866,8 @@ extern "C" int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, con
 
 extern "C" long long sca_linear_i8_workspace_bytes(long long M, int K) {
     if (M < 0 || K <= 0 || K > I8_MAX_K) return -1;
-    return one_launch(M, K) ? 0 : M * (pitch_of(K) + 4);
+    const long long pitch = pitch_of(K, true) > pitch_of(K, false) ? pitch_of(K, true) : pitch_of(K, false);
+    return one_launch(M, K) ? 0 : M * (pitch + 4);          // (N says which it is)
 }
 
 extern "C" int sca_linear_i8(const void* x, long long ldx, int dtype, const int8_t* wq, long long ldw, const float* sw,
@@ -877,7 +886,7 @@ extern "C" int sca_linear_i8(const void* x, long long ldx, int dtype, const int8
         else launch_direct<sca_f16>(a, st);
     } else {
         if (!ws || ((uintptr_t)ws & 15)) return -1;
-        const long long pitch = pitch_of(K);
+        const long long pitch = pitch_of(K, takes_direct(M, N, K));
         int8_t* q = (int8_t*)ws;
         float* scale = (float*)(q + M * pitch);
         quantize(x, ldx, dtype, M, K, q, pitch, scale, st);

@@ -314,7 +314,8 @@ class AdamW(torch.optim.Optimizer):
 
     The step number of each parameter lies on the device, so `step()` may be captured into a HIP graph after one ordinary
     call (lr and the other scalars are taken as they are at capture; a graph captured before `load_state_dict` goes on with the
-    states it was captured with; a second graph over gradients in other storage needs an ordinary call in between).  Gradients have their parameter's type and memory order;
+    states it was captured with; a second graph over gradients in other storage needs an ordinary call in between;
+    the optimizer has to outlive its graphs).  Gradients have their parameter's type and memory order;
     sparse gradients are refused.  One stream at a time may run an optimizer: work that uses it on another stream has to be
     ordered behind the first, as for any tensor."""
 

@@ -320,3 +320,24 @@ def test_int8_every_tail(ops, m, n, ks):
         one_m, one_n = torch.ones(m, device="cuda"), torch.ones(n, device="cuda")
         for x, w in ((xq, wq), (xq.contiguous(), wq.contiguous())):
             assert torch.equal(ops.int8_matmul(x, one_m, w, one_n), want), (k, x.stride())
+
+
+@pytest.mark.parametrize("k", [16, 112, 127, 128, 129, 1008, 2000, 2048, 8064, 8070])
+@pytest.mark.parametrize("m,n", [(1, 50), (2, 33), (3, 50), (100, 130), (700, 600)])
+def test_int8_linear_is_its_two_parts(ops, m, n, k):
+    """Quantized in the launch, in a workspace of whichever pitch, or by the caller: the same bits."""
+    x = matrix(m, k, torch.float32, m + k, "pitch")
+    wq, ws = ops.quantize_int8(torch.randn(n, k, device="cuda", generator=gen(3)))
+    bias = torch.randn(n, device="cuda", generator=gen(4))
+    q, s = ops.quantize_int8(x)
+    want = ops.int8_matmul(q, s, wq, ws, bias)
+    assert torch.equal(ops.int8_linear(x, wq, ws, bias), want)
+    # the workspace is as large as it says: guarded by a block of known bytes behind it
+    from scarches_amd import _lib
+    lib = _lib.load()
+    size = lib.sca_linear_i8_workspace_bytes(m, k)
+    buf = torch.full((size + 4096,), 85, dtype=torch.int8, device="cuda")
+    y = torch.empty(m, n, device="cuda")
+    _lib.check(lib.sca_linear_i8(x.data_ptr(), x.stride(0), 0, wq.data_ptr(), wq.stride(0), ws.data_ptr(), bias.data_ptr(), 0, m,
+                                 n, k, y.data_ptr(), 0, n, buf.data_ptr(), torch.cuda.current_stream().cuda_stream), "linear_i8")
+    assert torch.equal(y, want) and (buf[size:] == 85).all()
