@@ -191,7 +191,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
         rstd = a.stats[a.rows + r];
     };
     // 16-bit rows, whose arithmetic takes half as long as their loads: the next row is on its way meanwhile (16384 x 4000
-    // bf16: 81 instead of 100 us).  fp32 rows have no registers for it and run at the rate of a copy without.
+    // bf16: 81 instead of 100 us, with results through the caches).  fp32 rows have no registers for it and run at the rate of a copy without.
     constexpr bool AHEAD = sizeof(T) == 2 && HOLD;
     // (where rows meet at barriers, a wave without a row of its own goes along with zeros)
     constexpr bool TOGETHER = PER > 1 && TPR > 64;
