@@ -191,7 +191,8 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LnBwd a) {
         rstd = a.stats[a.rows + r];
     };
     // 16-bit rows, whose arithmetic takes half as long as their loads: the next row is on its way meanwhile (16384 x 4000
-    // bf16: 81 instead of 100 us, with results through the caches).  fp32 rows have no registers for it and run at the rate of a copy without.
+    // bf16: 81 instead of 100 us, with results through the caches).  fp32 rows have no registers for it and run at the rate
+    // of a copy without.
     constexpr bool AHEAD = sizeof(T) == 2 && HOLD;
     // (where rows meet at barriers, a wave without a row of its own goes along with zeros)
     constexpr bool TOGETHER = PER > 1 && TPR > 64;
@@ -396,7 +397,8 @@ BwdShape bwd_shape(long long rows, int n, int vec) {
     const int vecs = (n + vec - 1) / vec, v = 32 / vec;
     BwdShape s;
     const bool four = vecs > 128 && vecs <= 512 && (vecs > 256 || rows <= 8 * CUS);
-    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 && !four ? 64 : vecs <= 256 * v ? 256 : n <= max_held(vec, rows) ? 1024 : 0;
+    s.tpr = vecs <= 4 ? 4 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 && !four ? 64 : vecs <= 256 * v ? 256
+            : n <= max_held(vec, rows) ? 1024 : 0;
     s.nt = four ? 1024 : s.tpr > 64 ? s.tpr : rows * s.tpr <= 512 * CUS ? 256 : 512;
     if (s.tpr == 0) {
         const long long wide = (n + 256LL * vec - 1) / (256LL * vec), want = 4 * CUS / wide, most = (rows + 7) / 8;
@@ -448,8 +450,9 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
     else if (vecs <= 5120) FWD(1024, 5);
     else if (VEC == 4 && vecs <= 8192) FWD(1024, (VEC == 4 ? 8 : 5));
     else
-        hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(1024), 0, st, (const T*)x, ldx, rows, n,
-                           (const W*)w, (const W*)b, eps, (T*)y, ldy, stream, stats);
+        hipLaunchKernelGGL((ln_fwd_long_kernel<T, W>), dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)),
+                           dim3(1024), 0, st, (const T*)x, ldx, rows, n, (const W*)w, (const W*)b, eps, (T*)y, ldy, stream,
+                           stats);
 #undef FWD
 #undef FWD_MODE
     SCA_CHECK_LAUNCH();

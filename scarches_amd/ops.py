@@ -479,7 +479,8 @@ class AdamW(torch.optim.Optimizer):
         table = host.to(dev, non_blocking=True)
         at = table.data_ptr() + size
         return dict(key=key, grads=grads, captured=False, table=table, streams={_raw_stream(dev.index)}, entries=at,
-                    n=len(rows), chunks=at + len(entries), n_chunks=len(chunks), steps=steps, scratch=table.data_ptr(), index=dev.index)
+                    n=len(rows), chunks=at + len(entries), n_chunks=len(chunks), steps=steps, scratch=table.data_ptr(),
+                    index=dev.index)
 
     def _step(self, closure=None):
         loss = None
