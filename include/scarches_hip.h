@@ -400,7 +400,7 @@ int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_ada
  * 16 take the faster loads.  The forward product y = x W^T of the reference's nn.Linear layers
  * (scarches/models/trvae/modules.py:21-27) for serving.
  * sca_linear_i8: both in one call, y = x W^T + bias with x of dtype quantized on the way; one or two rows take one launch.
- * ws: scratch of sca_linear_i8_workspace_bytes(M, K) bytes, 16-byte aligned (0 bytes: may be NULL), any contents on entry,
+ * ws: scratch of sca_linear_i8_workspace_bytes(M, N, K) bytes, 16-byte aligned (0 bytes: may be NULL), any contents on entry,
  * not to be shared by calls that may overlap. */
 int sca_gemm_i8_max_k(void);
 int sca_quant_rows_i8(const void* x, long long ldx, int dtype, long long rows, int k, int8_t* q, long long ldq,
@@ -409,7 +409,7 @@ int sca_csr_quant_rows_i8(const int64_t* indptr, const int32_t* indices, const f
                           int G, int apply_log1p, int8_t* q, int ldq, float* scale, void* stream);
 int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, const int8_t* wq, long long ldw, const float* sw,
                 const void* bias, int btype, long long M, int N, int K, void* y, int ytype, long long ldy, void* stream);
-long long sca_linear_i8_workspace_bytes(long long M, int K);
+long long sca_linear_i8_workspace_bytes(long long M, int N, int K);
 int sca_linear_i8(const void* x, long long ldx, int dtype, const int8_t* wq, long long ldw, const float* sw,
                   const void* bias, int btype, long long M, int N, int K, void* y, int ytype, long long ldy, void* ws,
                   void* stream);

@@ -157,7 +157,7 @@ SIGNATURES = {
     "sca_quant_rows_i8": [P, LL, I, LL, I, P, LL, P, P],
     "sca_csr_quant_rows_i8": [P, P, P, P, I, I, I, P, I, P, P],
     "sca_gemm_i8": [P, LL, P, P, LL, P, P, I, LL, I, I, P, I, LL, P],
-    "sca_linear_i8_workspace_bytes": [LL, I],
+    "sca_linear_i8_workspace_bytes": [LL, I, I],
     "sca_linear_i8": [P, LL, I, P, LL, P, P, I, LL, I, I, P, I, LL, P, P],
     "sca_embed_lookup": [P, I, I, P, I, I, F, P, P, I, P],
     "sca_embed_scatter_add": [P, P, I, I, I, I, P, I, P, P],

@@ -75,16 +75,61 @@ __device__ __noinline__ void quantize_tiny(const T* x, int k, int8_t* q, float s
         q[c] = (int8_t)(int)fmin(fmax(rint((double)to_f32(x[c]) / (double)s), -127.0), 127.0);
 }
 
-// TPR threads per row, the row in registers: one read of 16 bytes a lane, one write.  Bound by memory.
-template <typename T, int TPR, int V, int MODE>
+// 16 bytes at p, of which `left` belong to the row of K bytes (what lies behind counts as 0).  The row's end is read as the 16
+// bytes that end with it, moved down: a byte at a time takes sixteen loads (a row shorter than that has no other way).
+__device__ __forceinline__ i32x4 load16(const int8_t* p, int left, int K) {
+    i32x4 v = {0, 0, 0, 0};
+    if (left >= 16) {
+        __builtin_memcpy(&v, p, 16);
+    } else if (left > 0 && K >= 16) {
+        uint64_t w[2];
+        __builtin_memcpy(w, p - (16 - left), 16);
+        const int shift = 8 * (16 - left);
+        const uint64_t lo = shift < 64 ? w[0] >> shift | w[1] << 1 << (63 - shift) : w[1] >> (shift - 64);
+        w[1] = shift < 64 ? w[1] >> shift : 0;
+        w[0] = lo;
+        __builtin_memcpy(&v, w, 16);
+    } else if (left > 0) {
+        int8_t b[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) b[i] = i < left ? p[i] : 0;
+        __builtin_memcpy(&v, b, 16);
+    }
+    return v;
+}
+
+// Rows of a weight to a pitch whose rows start 16-byte aligned, zeros behind them: workgroups `first` and up of the launch that
+// quantizes x beside it.
+struct AlignRows {
+    const int8_t* w; long long ldw;
+    int n, k;
+    int8_t* to; long long pitch;
+    unsigned first;
+};
+__device__ __forceinline__ unsigned blocks_left() { return gridDim.x; }
+__device__ __forceinline__ unsigned blocks_left(const AlignRows& a) { return a.first; }
+template <int NT>
+__device__ __forceinline__ void align_rows(const AlignRows& a) {
+    for (long long r = blockIdx.x - a.first; r < a.n; r += gridDim.x - a.first)
+        for (long long c = threadIdx.x * 16; c < a.pitch; c += NT * 16)
+            *(i32x4*)(a.to + r * a.pitch + c) = load16(a.w + r * a.ldw + c, a.k - (int)c, a.k);
+}
+
+// TPR threads per row, the row in registers: one read of 16 bytes a lane, one write.  Bound by memory.  Rows: nothing, or
+// AlignRows (arguments and a branch that are of no use cost 3 % of small calls).
+template <typename T, int TPR, int V, int MODE, typename... Rows>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void quant_rows_kernel(const T* __restrict__ x, long long ldx,
                                                                            long long rows, int k, int8_t* __restrict__ q,
-                                                                           long long ldq, float* __restrict__ scale) {
+                                                                           long long ldq, float* __restrict__ scale,
+                                                                           const Rows... al) {
     constexpr int VEC = vec_of<T>(), NT = TPR > 256 ? TPR : 256;
     __shared__ uint32_t scratch[16];
     const int t = threadIdx.x % TPR;
+    if constexpr (sizeof...(Rows) > 0) {
+        if (blockIdx.x >= blocks_left(al...)) return align_rows<NT>(al...);
+    }
     for (long long r = (long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR; r < rows;
-         r += (long long)gridDim.x * (NT / TPR)) {
+         r += (long long)blocks_left(al...) * (NT / TPR)) {
         const T* xr = x + r * ldx;
         raw_t x16[V] = {};
         float v[VEC];
@@ -218,29 +263,6 @@ __global__ __launch_bounds__(64) void csr_quant_rows_kernel(const int64_t* __res
     __syncthreads();
     for (int c = threadIdx.x * 16; c < ldq; c += 1024) *(i32x4*)(q + b * ldq + c) = *(const i32x4*)(row + c);
     if (threadIdx.x == 0) scale[b] = sc.s;
-}
-
-// 16 bytes at p, of which `left` belong to the row of K bytes (what lies behind counts as 0).  The row's end is read as the 16
-// bytes that end with it, moved down: a byte at a time takes sixteen loads (a row shorter than that has no other way).
-__device__ __forceinline__ i32x4 load16(const int8_t* p, int left, int K) {
-    i32x4 v = {0, 0, 0, 0};
-    if (left >= 16) {
-        __builtin_memcpy(&v, p, 16);
-    } else if (left > 0 && K >= 16) {
-        uint64_t w[2];
-        __builtin_memcpy(w, p - (16 - left), 16);
-        const int shift = 8 * (16 - left);
-        const uint64_t lo = shift < 64 ? w[0] >> shift | w[1] << 1 << (63 - shift) : w[1] >> (shift - 64);
-        w[1] = shift < 64 ? w[1] >> shift : 0;
-        w[0] = lo;
-        __builtin_memcpy(&v, w, 16);
-    } else if (left > 0) {
-        int8_t b[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) b[i] = i < left ? p[i] : 0;
-        __builtin_memcpy(&v, b, 16);
-    }
-    return v;
 }
 
 struct I8Args {
@@ -718,24 +740,35 @@ constexpr long long MAX_BLOCKS = 1 << 20;        // a launch holds fewer than 2^
 
 template <typename T, int TPR, int V>
 void launch_quant(const void* x, long long ldx, long long rows, int k, int8_t* q, long long ldq, float* scale,
-                  hipStream_t st) {
+                  AlignRows al, hipStream_t st) {
     constexpr int NT = TPR > 256 ? TPR : 256, PER = NT / TPR;
     const long long blocks = (rows + PER - 1) / PER;
-    const dim3 grid((unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS)), block(NT);
+    al.first = (unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS);
+    const dim3 grid(al.first + (al.n < 2048 ? al.n : 2048)), block(NT);
     const int mode = row_mode(k, vec_of<T>());
-    if (mode == ROW_FULL)
-        hipLaunchKernelGGL((quant_rows_kernel<T, TPR, V, ROW_FULL>), grid, block, 0, st, (const T*)x, ldx, rows, k, q, ldq, scale);
-    else if (mode == ROW_RAGGED)
-        hipLaunchKernelGGL((quant_rows_kernel<T, TPR, V, ROW_RAGGED>), grid, block, 0, st, (const T*)x, ldx, rows, k, q, ldq, scale);
-    else if constexpr (TPR == 16)
-        hipLaunchKernelGGL((quant_rows_kernel<T, TPR, V, ROW_TINY>), grid, block, 0, st, (const T*)x, ldx, rows, k, q, ldq, scale);
+#define QUANT_ROWS_OF(x) (const T*)x, ldx, rows, k, q, ldq, scale
+#define QUANT_MODE(MODE) \
+    hipLaunchKernelGGL((quant_rows_kernel<T, TPR, V, MODE>), grid, block, 0, st, QUANT_ROWS_OF(x))
+#define QUANT_ALIGN(MODE) \
+    hipLaunchKernelGGL((quant_rows_kernel<T, TPR, V, MODE, AlignRows>), grid, block, 0, st, QUANT_ROWS_OF(x), al)
+    if (TPR >= 64 && al.n) {
+        if constexpr (TPR >= 64) {
+            if (mode == ROW_FULL) QUANT_ALIGN(ROW_FULL);
+            else QUANT_ALIGN(ROW_RAGGED);
+        }
+    } else if (mode == ROW_FULL) QUANT_MODE(ROW_FULL);
+    else if (mode == ROW_RAGGED) QUANT_MODE(ROW_RAGGED);
+    else if constexpr (TPR == 16) QUANT_MODE(ROW_TINY);
+#undef QUANT_ROWS_OF
+#undef QUANT_ALIGN
+#undef QUANT_MODE
 }
 
 template <typename T>
 void quant_rows(const void* x, long long ldx, long long rows, int k, int8_t* q, long long ldq, float* scale,
-                hipStream_t st) {
+                const AlignRows& al, hipStream_t st) {
     const int vecs = (k + vec_of<T>() - 1) / vec_of<T>();
-#define QUANT(TPR, V) return launch_quant<T, TPR, V>(x, ldx, rows, k, q, ldq, scale, st)
+#define QUANT(TPR, V) return launch_quant<T, TPR, V>(x, ldx, rows, k, q, ldq, scale, al, st)
     // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory.
     if (vecs <= 16) QUANT(16, 1);
     if (vecs <= 64) QUANT(64, 1);
@@ -785,7 +818,9 @@ void launch_direct(I8Args a, hipStream_t st) {
 //   509 x 282 x 1972    8.3 / 7.5 / 12.6 / 28         4096 x 4096 x 4096    - / 156 / 84 / 69
 //   1000 x 250 x 300    6.1 / 5.4 / 8.1 / -           65536 x 64 x 512      40 / 17 / 10.9 / 16.1
 // Direct: one workgroup per CU at most, or a few with short rows (or single cells, whose x is read from the caches); 64: no
-// more tiles than CUs.  Larger tiles read less; they need about one tile per CU, and little of it lost behind the edges.
+// more tiles than CUs.  Larger tiles read less; they need about one tile per CU, little of it lost behind the edges, and no
+// last run over the chip with few of them (21986 x 543 x 608, 258 tiles of 256: 38 us, 25 in tiles of 128).  Over 60 sizes
+// drawn between 2e9 and 1.3e11 products the rule takes 1 % longer than the best of the three.
 constexpr int CUS = 256;
 bool takes_direct(long long M, int N, int K) {
     const long long tiles = ((M + 15) / 16) * ((N + 15LL) / 16);
@@ -795,15 +830,18 @@ bool takes_direct(long long M, int N, int K) {
 void gemm_i8(const I8Args& a, hipStream_t st) {
     const bool aligned = !(((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.ldx | (uintptr_t)a.ldw) & 15);
     auto tiles = [&](int b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
+    auto runs = [&](int b, int per_cu) { return (tiles(b) + per_cu * CUS - 1) / (per_cu * CUS); };
     if (takes_direct(a.M, a.N, a.K)) {
         launch_direct<int8_t>(a, st);
-    } else if (aligned && tiles(256) >= 192 && 16 * tiles(256) <= 5 * tiles(128)) {
+    } else if (aligned && tiles(256) >= 192 && 16 * tiles(256) <= 5 * tiles(128) && 11 * runs(256, 1) * CUS <= 15 * tiles(256)) {
         launch_tile<256, 256, 2, 4, 64, 4, 1, true>(a, st);
-    } else if (tiles(64) > CUS) {
-        if (aligned) launch_tile<128, 128, 2, 2, 64, 4, 1, true>(a, st);
-        else launch_tile<128, 128, 2, 2, 64, 4, 1, false>(a, st);
+    } else if (aligned) {
+        if (tiles(64) > CUS) launch_tile<128, 128, 2, 2, 64, 4, 1, true>(a, st);
+        else launch_tile<64, 64, 2, 2, 128, 2, 4, true>(a, st);
     } else {
-        if (aligned) launch_tile<64, 64, 2, 2, 128, 2, 4, true>(a, st);
+        // (what a run of tiles over the chip takes, two of the larger ones per CU, fitted to 60 sizes: within 1 % of the better)
+        if (runs(128, 2) * (4 + 0.0104 * a.K) < runs(64, 1) * (3.25 + 0.0028 * a.K))
+            launch_tile<128, 128, 2, 2, 64, 4, 1, false>(a, st);
         else launch_tile<64, 64, 2, 2, 128, 2, 4, false>(a, st);
     }
 }
@@ -812,10 +850,10 @@ constexpr int MAX_N = 0x7ffff000;               // (columns are counted in 32 bi
 constexpr int I8_MAX_K = (1 << 17) - 1;         // 2^17 products of -128 * -128 would pass int32
 
 void quantize(const void* x, long long ldx, int dtype, long long rows, int k, int8_t* q, long long ldq, float* scale,
-              hipStream_t st) {
-    if (dtype == SCA_F32) quant_rows<float>(x, ldx, rows, k, q, ldq, scale, st);
-    else if (dtype == SCA_BF16) quant_rows<sca_bf16>(x, ldx, rows, k, q, ldq, scale, st);
-    else quant_rows<sca_f16>(x, ldx, rows, k, q, ldq, scale, st);
+              hipStream_t st, const AlignRows& al = AlignRows{}) {
+    if (dtype == SCA_F32) quant_rows<float>(x, ldx, rows, k, q, ldq, scale, al, st);
+    else if (dtype == SCA_BF16) quant_rows<sca_bf16>(x, ldx, rows, k, q, ldq, scale, al, st);
+    else quant_rows<sca_f16>(x, ldx, rows, k, q, ldq, scale, al, st);
 }
 bool one_launch(long long M, int K) { return M <= QUANT_ROWS && K <= QUANT_K - 128; }
 // Pitch of the rows that sca_linear_i8 quantizes for itself.  Tiles want whole cache lines (128 x 128 tiles, 16384 x 256 x
@@ -824,6 +862,10 @@ bool one_launch(long long M, int K) { return M <= QUANT_ROWS && K <= QUANT_K - 1
 long long pitch_of(int K, bool direct) {
     return direct ? (((long long)K + 15) / 16 | 1) * 16 : ((long long)K + 127) & ~127LL;
 }
+// A weight whose rows are not 16-byte aligned is copied to rows that are, in the launch that quantizes x, where that is
+// little work beside the product (us of the product with rows as they are / aligned: 1071 x 1338 x 2217 23 / 14, 20030 x 1294 x
+// 1636 90 / 67, 665 x 1621 x 6263 43 / 28; but 22267 x 1920 x 68 27.5 / 29.2, and 213 x 2051 x 7874 24 / 19 with 6 for the copy).
+bool worth_aligning(long long M, int N, int K) { return M >= 512 && K >= 512 && K <= 32768 && !takes_direct(M, N, K); }
 
 }  // namespace
 
@@ -864,10 +906,10 @@ extern "C" int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, con
     return 0;
 }
 
-extern "C" long long sca_linear_i8_workspace_bytes(long long M, int K) {
-    if (M < 0 || K <= 0 || K > I8_MAX_K) return -1;
-    const long long pitch = pitch_of(K, true) > pitch_of(K, false) ? pitch_of(K, true) : pitch_of(K, false);
-    return one_launch(M, K) ? 0 : M * (pitch + 4);          // (N says which it is)
+extern "C" long long sca_linear_i8_workspace_bytes(long long M, int N, int K) {
+    if (M < 0 || N < 0 || N > MAX_N || K <= 0 || K > I8_MAX_K) return -1;
+    if (one_launch(M, K)) return 0;
+    return M * (pitch_of(K, takes_direct(M, N, K)) + 4) + (worth_aligning(M, N, K) ? N * pitch_of(K, false) : 0);
 }
 
 extern "C" int sca_linear_i8(const void* x, long long ldx, int dtype, const int8_t* wq, long long ldw, const float* sw,
@@ -889,7 +931,15 @@ extern "C" int sca_linear_i8(const void* x, long long ldx, int dtype, const int8
         const long long pitch = pitch_of(K, takes_direct(M, N, K));
         int8_t* q = (int8_t*)ws;
         float* scale = (float*)(q + M * pitch);
-        quantize(x, ldx, dtype, M, K, q, pitch, scale, st);
+        AlignRows al = {};
+        if (worth_aligning(M, N, K)) {
+            scale = (float*)(q + M * pitch + N * pitch_of(K, false));
+            if (((uintptr_t)wq | (uintptr_t)ldw) & 15) {
+                al = AlignRows{wq, ldw, N, K, q + M * pitch, pitch_of(K, false), 0};
+                a.w = al.to; a.ldw = al.pitch;
+            }
+        }
+        quantize(x, ldx, dtype, M, K, q, pitch, scale, st, al);
         a.x = q; a.ldx = pitch; a.sx = scale;
         gemm_i8(a, st);
     }

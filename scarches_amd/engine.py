@@ -2208,7 +2208,7 @@ class CVAEEngine:
             _lib.check(raw.sca_gemm_i8(q.data_ptr(), q.stride(0), sx.data_ptr(), wq.data_ptr(), wq.stride(0), scale.data_ptr(),
                                        None, 0, B, ly.n_out, ly.n_in, slab.data_ptr(), 0, ly.n_out, st), "gemm_i8")
             return slab.data_ptr(), 1, B * ly.n_out
-        size = raw.sca_linear_i8_workspace_bytes(B, ly.n_in)
+        size = raw.sca_linear_i8_workspace_bytes(B, ly.n_out, ly.n_in)
         scratch = torch.empty(size, dtype=torch.int8, device=self.device) if size else None
         _lib.check(raw.sca_linear_i8(a, ly.n_in, 0, wq.data_ptr(), wq.stride(0), scale.data_ptr(), None, 0, B, ly.n_out,
                                      ly.n_in, slab.data_ptr(), 0, ly.n_out, _lib.ptr(scratch), st), "linear_i8")

@@ -276,7 +276,7 @@ def int8_linear(x, wq, w_scale, bias: Optional[torch.Tensor] = None, out_dtype=N
     n = wq.shape[0]
     y = x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
     if rows and n:
-        size = _fn("sca_linear_i8_workspace_bytes")(rows, k)
+        size = _fn("sca_linear_i8_workspace_bytes")(rows, n, k)
         ws = x.new_empty((size,), dtype=torch.int8) if size else None
         _call(index, "sca_linear_i8", x2.data_ptr(), ldx, xcode, wq.data_ptr(), ldw, w_scale.data_ptr(), _lib.ptr(bias),
               bcode, rows, n, k, y.data_ptr(), code, n, _lib.ptr(ws))

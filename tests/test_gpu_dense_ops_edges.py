@@ -335,9 +335,23 @@ def test_int8_linear_is_its_two_parts(ops, m, n, k):
     # the workspace is as large as it says: guarded by a block of known bytes behind it
     from scarches_amd import _lib
     lib = _lib.load()
-    size = lib.sca_linear_i8_workspace_bytes(m, k)
+    size = lib.sca_linear_i8_workspace_bytes(m, n, k)
     buf = torch.full((size + 4096,), 85, dtype=torch.int8, device="cuda")
     y = torch.empty(m, n, device="cuda")
     _lib.check(lib.sca_linear_i8(x.data_ptr(), x.stride(0), 0, wq.data_ptr(), wq.stride(0), ws.data_ptr(), bias.data_ptr(), 0, m,
                                  n, k, y.data_ptr(), 0, n, buf.data_ptr(), torch.cuda.current_stream().cuda_stream), "linear_i8")
     assert torch.equal(y, want) and (buf[size:] == 85).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(512, 700, 512), (513, 1025, 1001), (2000, 300, 2049), (600, 2100, 777), (900, 333, 20001)])
+def test_int8_linear_aligns_the_weight(ops, m, n, k, dtype):
+    """Weights that lie packed, with an odd pitch or from an odd address give the bits of the padded one."""
+    x = matrix(m, k, dtype, m + k, "odd")
+    wq, ws = ops.quantize_int8(torch.randn(n, k, device="cuda", generator=gen(3)))
+    q, s = ops.quantize_int8(x)
+    want = ops.int8_matmul(q, s, wq, ws, None, dtype)
+    buf = torch.full((n * (k + 7) + 1,), -128, dtype=torch.int8, device="cuda")
+    for w in (wq, wq.contiguous(), torch.as_strided(buf, (n, k), (k + 7, 1), 1).copy_(wq),
+              wq.t().contiguous().t()):
+        assert torch.equal(ops.int8_linear(x, w, ws), want), w.stride()

@@ -111,8 +111,9 @@ def test_entry_points_check_their_arguments():
     for i, bad in ((0, None), (1, -1), (2, 3), (3, None), (4, 7), (5, None), (7, 1), (8, -1), (9, -1), (10, 0), (11, None), (12, -1),
                    (13, 4), (14, None), (14, a + 8)):
         assert lib.sca_linear_i8(*ok[:i], bad, *ok[i + 1:]) == -1, i
-    assert lib.sca_linear_i8_workspace_bytes(40, 8) == 40 * 132 and lib.sca_linear_i8_workspace_bytes(1, 8) == 0
-    assert lib.sca_linear_i8_workspace_bytes(-1, 8) == -1 and lib.sca_linear_i8_workspace_bytes(1, 1 << 17) == -1
+    assert lib.sca_linear_i8_workspace_bytes(40, 5, 8) >= 40 * (8 + 4) and lib.sca_linear_i8_workspace_bytes(1, 5, 8) == 0
+    assert lib.sca_linear_i8_workspace_bytes(-1, 5, 8) == lib.sca_linear_i8_workspace_bytes(1, -1, 8) == -1
+    assert lib.sca_linear_i8_workspace_bytes(1, 5, 1 << 17) == -1
     ok = (a, 1, a, 1, 32, None, 0, 1e-3, 0.9, 0.999, 1e-8, 0, a, None)
     for i, bad in ((0, None), (1, -1), (2, None), (3, -1), (4, 16), (6, -1), (8, 1.0), (9, -0.1), (10, -1.0), (12, None), (12, a + 8)):
         assert lib.sca_adamw_step(*ok[:i], bad, *ok[i + 1:]) == -1, i
