@@ -694,6 +694,7 @@ def test_adamw_under_graph_capture(ops, bits):
     other = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="before the capture"):
         with torch.cuda.graph(other):
+            grads[0].zero_()                    # (never replayed; no graph here is left without a node)
             b.step()
 
 
