@@ -18,6 +18,7 @@ from typing import Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.optim import optimizer as _optimizer
 
 from . import _lib
@@ -46,8 +47,16 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
+def _no_tangents(tensors):
+    """A dual tensor does not require grad: its tangent would be lost without a word (and read as zero)."""
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("scarches_amd.ops has no forward-mode derivatives (a tensor of the call carries a tangent)")
+
+
 def _same_device(*tensors) -> int:
-    """The number of the one HIP device that all tensors (or None) are on."""
+    """The number of the one HIP device that all tensors (or None) are on.  Every operator asks before it launches anything."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents(tensors)
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != index:
@@ -171,12 +180,15 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """Layer norm over the last dimension of x with optional weight and bias [n]; gradients of x, weight and bias.
+    """Layer norm over the last dimension of x with optional weight and bias [n]; gradients of x, weight and bias (reverse mode,
+    once; a tensor with a forward-mode tangent is refused here and by every operator of this module).
 
     Statistics and sums are held in float32 whatever x's type, and each result is rounded once.  A row with NaN or an
     infinity gives NaN in that row (and in the weight's gradient) only."""
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
+        if _forward_ad._current_level >= 0:         # (what apply() calls does not see tangents)
+            _no_tangents((x, weight, bias))
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_fwd(x, weight, bias, eps)[0]
 
