@@ -9,7 +9,7 @@ with a scale per row and per output channel for serving.
 
 All arithmetic runs in the HIP kernels behind include/scarches_hip.h (sca_layernorm_*, sca_adamw_step, sca_quant_rows_i8,
 sca_gemm_i8) on the current stream of the tensors' device; there is no CPU fallback.  Wrong shapes and types raise ValueError
-/ TypeError before anything is launched.
+/ TypeError before anything is launched; torch.jit.trace, make_fx, fake tensors and forward-mode tangents RuntimeError.
 """
 from __future__ import annotations
 
@@ -47,6 +47,16 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
+def _recording() -> bool:
+    """True inside torch.jit.trace, make_fx and on fake tensors: what they record of an operator is the allocation of its
+    results, and what they replay computes nothing.  (Under torch.compile an operator is a graph break and runs as ever.)"""
+    if torch._C._is_tracing():
+        return True
+    key = torch._C._TorchDispatchModeKey
+    return torch._C._len_torch_dispatch_stack() > 0 and (torch._C._get_dispatch_mode(key.PROXY) is not None
+                                                         or torch._C._get_dispatch_mode(key.FAKE) is not None)
+
+
 def _no_tangents(tensors):
     """A dual tensor does not require grad: its tangent would be lost without a word (and read as zero)."""
     if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
@@ -57,6 +67,8 @@ def _same_device(*tensors) -> int:
     """The number of the one HIP device that all tensors (or None) are on.  Every operator asks before it launches anything."""
     if _forward_ad._current_level >= 0:
         _no_tangents(tensors)
+    if _recording():
+        raise RuntimeError("the kernels of scarches_amd.ops are launched through addresses, which a trace does not record")
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != index:

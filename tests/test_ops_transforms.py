@@ -11,7 +11,7 @@ def t(*shape, dtype=torch.float32):
     return torch.ones(*shape, dtype=dtype)
 
 
-W8 = torch.ones(5, 4, dtype=torch.int8)
+W8, W4 = torch.ones(5, 4, dtype=torch.int8), torch.ones(4, 4, dtype=torch.int8)
 # the operator as a function of one fp32 tensor [3, 4] that it differentiates, or should
 CALLS = {
     "layer_norm": lambda x: ops.layer_norm(x, t(4), t(4)),
@@ -24,7 +24,7 @@ CALLS = {
     "quantize_int8": lambda x: ops.quantize_int8(x),
     "int8_matmul": lambda x: ops.int8_matmul(t(3, 4, dtype=torch.int8), x[:, 0].contiguous(), W8, t(5)),
     "int8_linear": lambda x: ops.int8_linear(x, W8, t(5)),
-    "int8_linear bias": lambda x: ops.int8_linear(t(3, 4), W8[:4], t(4), x[0]),
+    "int8_linear bias": lambda x: ops.int8_linear(t(3, 4), W4, t(4), x[0]),
 }
 
 
@@ -43,3 +43,40 @@ def test_a_level_without_tangents_is_none():
             ops.layer_norm(t(3, 4), t(4), t(4))
         with pytest.raises(RuntimeError, match="HIP device"):
             ops.int8_linear(t(3, 4), W8, t(5))
+
+
+RECORDED = {k: f for k, f in CALLS.items() if "learns" not in k}
+
+
+@pytest.mark.parametrize("name", RECORDED)
+def test_traces_are_refused(name):
+    """What torch.jit.trace and make_fx record of a call is an allocation: its replays would return what lies there."""
+    def f(x):
+        out = RECORDED[name](x * 1)
+        return out[0] if isinstance(out, tuple) else out
+    with pytest.raises(RuntimeError, match="trace does not record"):
+        torch.jit.trace(f, (t(3, 4),))
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(RuntimeError, match="trace does not record"):
+            make_fx(f, tracing_mode=mode)(t(3, 4))
+
+
+def test_fake_tensors_are_refused():
+    """Their addresses are 0: nothing may be launched on them, the optimizer's table of addresses included."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        with pytest.raises(RuntimeError, match="trace does not record"):
+            ops.layer_norm(t(3, 4), t(4), t(4))
+        p = t(3)
+        p.grad = t(3)
+        with pytest.raises(RuntimeError, match="trace does not record"):
+            ops.AdamW([p]).step()
+
+
+def test_other_modes_pass():
+    """A mode that only looks on (the counter of flops) is none of these."""
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            ops.layer_norm(t(3, 4), t(4), t(4))
