@@ -4,7 +4,7 @@ with a scale per row and per output channel for serving.
 
     y = ops.layer_norm(x, weight, bias)                          # differentiable
     opt = ops.AdamW(net.parameters(), lr=1e-3, state_bits=8)     # torch.optim.Optimizer
-    wq, ws = ops.quantize_int8(weight)                           # once
+    wq, ws = ops.quantize_int8(weight.detach())                  # once
     y = ops.int8_linear(x, wq, ws, bias)                         # per request
 
 All arithmetic runs in the HIP kernels behind include/scarches_hip.h (sca_layernorm_*, sca_adamw_step, sca_quant_rows_i8,
@@ -212,11 +212,13 @@ _PAD_K = 128        # pitch of quantized rows: a multiple of the product's k ste
 def quantize_int8(x):
     """(q, scale) of the rows of x [..., k]: int8 q [..., k] and float32 scale [...] with x ~ q * scale[..., None], scale =
     max |x| / 127 of the row.  q is a view of rows padded with zeros to a multiple of 128 bytes, as `int8_matmul` reads them
-    fastest.  A row of zeros has scale 0; a row with NaN or an infinity has scale NaN, and so have results computed from it."""
+    fastest.  A row of zeros has scale 0; a row with NaN or an infinity has scale NaN, and so have results computed from it.
+    No gradient: a parameter is quantized under torch.no_grad() or detached."""
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"quantize_int8 needs rows of at least one value, got shape {tuple(x.shape)}")
     _check_width(x.shape[-1])
     code = _dtype_code(x, "x")
+    _no_grad(x)
     index = _same_device(x)
     x2, rows, ldx = _rows(x)
     k = x.shape[-1]
@@ -251,7 +253,7 @@ def _i8_check(k, wq, w_scale, bias, out_dtype):
 
 def _no_grad(*tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the 8-bit integer product is for serving and has no gradient: call it under torch.no_grad()")
+        raise RuntimeError("the 8-bit integer operators are for serving and have no gradient: call them under torch.no_grad()")
 
 
 def _weight_rows(wq):

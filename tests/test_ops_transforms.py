@@ -80,3 +80,13 @@ def test_other_modes_pass():
     with FlopCounterMode(display=False):
         with pytest.raises(RuntimeError, match="HIP device"):
             ops.layer_norm(t(3, 4), t(4), t(4))
+
+
+def test_quantizing_what_learns_is_refused():
+    """As the product does: the scale depends on x, and its gradient would be lost."""
+    w = t(3, 4).requires_grad_()
+    with pytest.raises(RuntimeError, match="have no gradient"):
+        ops.quantize_int8(w)
+    for call in (lambda: ops.quantize_int8(w.detach()), lambda: torch.no_grad()(ops.quantize_int8)(w)):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call()
