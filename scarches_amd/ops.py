@@ -431,10 +431,22 @@ class AdamW(torch.optim.Optimizer):
         return sd
 
     def load_state_dict(self, state_dict):
-        """Take up the states of a `state_dict()` of this class with the same state_bits, or (32 bits) of torch.optim.AdamW."""
+        """Take up the states of a `state_dict()` of this class with the same state_bits, or (32 bits) of torch.optim.AdamW.
+        ValueError for a run whose rule is another one (amsgrad, maximize, torch.optim.Adam's coupled decay) or whose states
+        are not these: nothing is changed then."""
+        for group in state_dict["param_groups"]:
+            if not {"lr", "betas", "eps", "weight_decay"} <= set(group):
+                raise ValueError("the state dict is of another optimizer: its groups lack lr, betas, eps or weight_decay")
+            for key in ("amsgrad", "maximize"):
+                if group.get(key):
+                    raise ValueError(f"the state dict is of a run with {key}=True, which this optimizer does not have")
+            if not group.get("decoupled_weight_decay", True):
+                raise ValueError("the state dict is of torch.optim.Adam, whose weight decay is part of the gradient")
+            if any(isinstance(x, torch.Tensor) for x in (group["lr"], *group["betas"])):
+                raise ValueError("the state dict's lr and betas must be numbers")
         keys = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
         for st in state_dict["state"].values():
-            if not keys <= set(st) or ("exp_avg_scale" in st) != (self.state_bits == 8):
+            if set(st) - {"step"} != keys:
                 raise ValueError(f"the state dict holds {sorted(st)}, this optimizer keeps {self.state_bits}-bit states")
         super().load_state_dict(state_dict)
         self._plans = {}

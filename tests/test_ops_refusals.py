@@ -148,3 +148,44 @@ def test_csr_rows_entry_point():
         assert lib.sca_csr_quant_rows_i8(*ok[:i], bad, *ok[i + 1:]) == -1, i
     assert lib.sca_csr_quant_rows_i8(a, a, a, None, 4, 65537, 1, a, 65552, a, None) == -2       # wider than the LDS
     assert lib.sca_csr_quant_rows_i8(a, a, a, None, 0, 100, 1, a, 112, a, None) == 0
+
+
+def torch_states(cls, steps=2, **kw):
+    p = t(4, 3).requires_grad_()
+    opt = cls([p], lr=1e-2, weight_decay=0.1, **kw)
+    for _ in range(steps):
+        p.grad = t(4, 3) + 0.5
+        opt.step()
+    return opt.state_dict()
+
+
+@pytest.mark.parametrize("cls,kw,error", [
+    (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"), (torch.optim.AdamW, dict(maximize=True), "maximize"),
+    (torch.optim.AdamW, dict(amsgrad=True, steps=0), "amsgrad"), (torch.optim.Adam, dict(), "torch.optim.Adam,"),
+    (torch.optim.SGD, dict(momentum=0.9), "another optimizer")])
+def test_adamw_takes_up_no_other_rule(cls, kw, error):
+    """A state dict whose next step would not be this class's: refused, with the optimizer as it was."""
+    opt = ops.AdamW([t(4, 3)], lr=0.3)
+    sd = torch_states(cls, **kw)
+    with pytest.raises(ValueError, match=error):
+        opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] == 0.3 and not opt.state
+
+
+def test_adamw_takes_up_torch_states():
+    sd = torch_states(torch.optim.AdamW)
+    p = t(4, 3)
+    opt = ops.AdamW([p], lr=0.3)
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] == 1e-2 and opt.state_dict()["state"][0]["step"] == 2
+    assert torch.equal(opt.state[p]["exp_avg_sq"], sd["state"][0]["exp_avg_sq"])
+    for change in (lambda s: s["state"][0].pop("exp_avg"), lambda s: s["state"][0].update(max_exp_avg_sq=t(4, 3)),
+                   lambda s: s["param_groups"][0].update(lr=torch.tensor(0.1)),
+                   lambda s: s["param_groups"][0].update(betas=(torch.tensor(0.9), 0.999))):
+        other = torch_states(torch.optim.AdamW)
+        change(other)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other)
+    with pytest.raises(ValueError, match="8-bit states"):
+        ops.AdamW([p], state_bits=8).load_state_dict(sd)
+    assert opt.state_dict()["state"][0]["step"] == 2
