@@ -528,7 +528,7 @@ class AdamW(torch.optim.Optimizer):
         scales = self.state_bits == 8
         for gi, group in enumerate(self.param_groups):
             # what the table was made of: addresses, sizes, types and layouts
-            key, grads, bits, mask = [group["weight_decay"]], [], 0, 0
+            key, grads, taken, bits, mask = [group["weight_decay"]], [], [], 0, 0
             for p in group["params"]:
                 g = p.grad
                 mask <<= 1
@@ -540,6 +540,7 @@ class AdamW(torch.optim.Optimizer):
                     self._init_state(p)
                 at = g.data_ptr()
                 grads.append(at)
+                taken.append(p)
                 bits |= at
                 key += (p.data_ptr(), p.numel(), p.dtype, g.dtype, g.is_contiguous() or g.stride(),
                         st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
@@ -576,6 +577,8 @@ class AdamW(torch.optim.Optimizer):
             b1, b2 = group["betas"]
             _call(plan["index"], "sca_adamw_step", plan["entries"], plan["n"], plan["chunks"], plan["n_chunks"],
                   self.state_bits, None, t or 0, group["lr"], b1, b2, group["eps"], self.seed, plan["scratch"])
+            # the kernel writes through addresses: autograd has to hear that what it may have saved is not there any more
+            torch.autograd.graph.increment_version(taken)
         return loss
 
     # torch wraps step() to run its hooks and to be seen by the profiler, which takes 6 us: here only where one is wanted
