@@ -572,11 +572,15 @@ class AdamW(torch.optim.Optimizer):
                 if moved:   # the table changes when the graph runs, not now
                     del self._plans[gi]
                 t = None
-            t = None if t is None else t + 1
-            self._host_steps[gi] = (t, None if t is None else mask)
+            if t is None:
+                self._host_steps[gi] = (None, None)
+            else:
+                t += 1
             b1, b2 = group["betas"]
             _call(plan["index"], "sca_adamw_step", plan["entries"], plan["n"], plan["chunks"], plan["n_chunks"],
                   self.state_bits, None, t or 0, group["lr"], b1, b2, group["eps"], self.seed, plan["scratch"])
+            if t is not None:       # (a call that raised has counted nothing)
+                self._host_steps[gi] = (t, mask)
             # the kernel writes through addresses: autograd has to hear that what it may have saved is not there any more
             torch.autograd.graph.increment_version(taken)
         return loss
