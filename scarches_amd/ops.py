@@ -335,7 +335,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits=32: `exp_avg`, `exp_avg_sq` in float32 whatever the parameter's type.
     state_bits=8: `exp_avg` float8_e4m3fn and `exp_avg_sq` float8_e5m2, each with one float32 power of two per 256 elements
     (`exp_avg_scale`, `exp_avg_sq_scale`): 2.03 bytes per value instead of 8.  Rounding to 8 bits is stochastic, from a
-    generator of (seed, parameter, element, step): the same seed gives the same run.  A gradient that is not finite makes
+    generator of (seed, parameter, element, step): the same seed gives the same run, and a state dict holds it.  A gradient that is not finite makes
     the moments of its 256 elements NaN.
 
     The step number of each parameter lies on the device, so `step()` may be captured into a HIP graph after one ordinary
@@ -419,8 +419,11 @@ class AdamW(torch.optim.Optimizer):
                 self._host_steps[gi] = (int(step), None)
 
     def state_dict(self):
-        """torch's layout; every parameter's state has `step` as a whole number (read from the device)."""
+        """torch's layout; every parameter's state has `step` as a whole number (read from the device), and with 8-bit states
+        every group the `seed` of the rounding."""
         sd = super().state_dict()
+        if self.state_bits == 8:
+            sd["param_groups"] = [dict(group, seed=self.seed) for group in sd["param_groups"]]
         for gi, packed in enumerate(sd["param_groups"]):
             if gi not in self._steps:
                 continue
@@ -432,6 +435,7 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Take up the states of a `state_dict()` of this class with the same state_bits, or (32 bits) of torch.optim.AdamW.
+        8-bit states bring the seed of their rounding along, so that the run goes on as it would have.
         ValueError for a run whose rule is another one (amsgrad, maximize, torch.optim.Adam's coupled decay) or whose states
         are not these: nothing is changed then."""
         for group in state_dict["param_groups"]:
@@ -448,7 +452,14 @@ class AdamW(torch.optim.Optimizer):
         for st in state_dict["state"].values():
             if set(st) - {"step"} != keys:
                 raise ValueError(f"the state dict holds {sorted(st)}, this optimizer keeps {self.state_bits}-bit states")
+        seeds = {int(group["seed"]) for group in state_dict["param_groups"] if "seed" in group}
+        if len(seeds) > 1:
+            raise ValueError(f"the state dict's groups hold different seeds: {sorted(seeds)}")
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            group.pop("seed", None)
+        if seeds:
+            self.seed = seeds.pop()
         self._plans = {}
         for gi, (group, packed) in enumerate(zip(self.param_groups, state_dict["param_groups"])):
             steps = []

@@ -82,3 +82,27 @@ def test_a_failed_call_that_the_device_counts(calls, monkeypatch):
     q.grad = None
     opt.step()
     assert step_number(calls[-1]) == 0
+
+
+def test_the_state_dict_holds_the_seed(calls):
+    """A run that is taken up by an optimizer of another seed goes on with its own: the rounding of its states hangs on it."""
+    p, q = param(300), param(300)
+    opt, other = ops.AdamW([p], state_bits=8, seed=2 ** 63 + 9), ops.AdamW([q], state_bits=8)
+    p.grad = q.grad = torch.ones(300)
+    opt.step()
+    sd = opt.state_dict()
+    other.load_state_dict(sd)
+    other.step()
+    assert other.seed == 2 ** 63 + 9 and calls[-1][1][11] == 2 ** 63 + 9
+    assert "seed" not in other.param_groups[0] and other.state_dict()["param_groups"] == sd["param_groups"]
+    for group in sd["param_groups"]:
+        del group["seed"]                                   # saved before there was one: the constructor's
+    third = ops.AdamW([param(300)], state_bits=8, seed=4)
+    third.load_state_dict(sd)
+    assert third.seed == 4
+    two = ops.AdamW([dict(params=[param(3)]), dict(params=[param(3)])], state_bits=8)
+    sd = two.state_dict()
+    sd["param_groups"][1]["seed"] = 1
+    with pytest.raises(ValueError, match="different seeds"):
+        two.load_state_dict(sd)
+    assert "seed" not in ops.AdamW([param(3)]).state_dict()["param_groups"][0]
