@@ -413,7 +413,9 @@ class AdamW(torch.optim.Optimizer):
         """Set the number of steps that every parameter has behind it (a run taken up from states of another program)."""
         if int(step) < 0:
             raise ValueError(f"a parameter cannot have {step} steps behind it")
-        for gi in range(len(self.param_groups)):
+        for gi, group in enumerate(self.param_groups):
+            if not group["params"]:
+                continue
             self._group_steps(gi).fill_(int(step))
             if self._host_steps.get(gi, (0,))[0] is not None:
                 self._host_steps[gi] = (int(step), None)
@@ -463,6 +465,8 @@ class AdamW(torch.optim.Optimizer):
         self._plans = {}
         for gi, (group, packed) in enumerate(zip(self.param_groups, state_dict["param_groups"])):
             steps = []
+            if not group["params"]:
+                continue
             for p, pid in zip(group["params"], packed["params"]):
                 st = state_dict["state"].get(pid)
                 steps.append(int(st.get("step", 0)) if st else 0)

@@ -106,3 +106,16 @@ def test_the_state_dict_holds_the_seed(calls):
     with pytest.raises(ValueError, match="different seeds"):
         two.load_state_dict(sd)
     assert "seed" not in ops.AdamW([param(3)]).state_dict()["param_groups"][0]
+
+
+def test_a_group_without_parameters(calls):
+    """torch allows one (all of its parameters frozen away, say): it takes no part in anything."""
+    p = param(3)
+    p.grad = torch.ones(3)
+    opt = ops.AdamW([dict(params=[]), dict(params=[p], lr=0.5)])
+    opt.set_step(7)
+    opt.step()
+    assert len(calls) == 1 and step_number(calls[0]) == 8
+    other = ops.AdamW([dict(params=[]), dict(params=[param(3)])])
+    other.load_state_dict(opt.state_dict())
+    assert other.param_groups[1]["lr"] == 0.5 and other._host_steps == {1: (7, 1)}
