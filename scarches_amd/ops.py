@@ -557,8 +557,8 @@ class AdamW(torch.optim.Optimizer):
                 grads.append(at)
                 taken.append(p)
                 bits |= at
-                key += (p.data_ptr(), p.numel(), p.dtype, g.dtype, g.is_contiguous() or g.stride(),
-                        st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
+                key += (p.data_ptr(), p.numel(), g.numel(), p.dtype, g.dtype,
+                        p.is_contiguous() and g.is_contiguous() or (p.stride(), g.stride()), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
                 if scales:
                     key += (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr())
             if not grads:           # (nobody takes a step: nothing to count)

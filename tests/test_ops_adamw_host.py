@@ -119,3 +119,33 @@ def test_a_group_without_parameters(calls):
     other = ops.AdamW([dict(params=[]), dict(params=[param(3)])])
     other.load_state_dict(opt.state_dict())
     assert other.param_groups[1]["lr"] == 0.5 and other._host_steps == {1: (7, 1)}
+
+
+def test_tensors_that_change_in_place(calls):
+    """Behind .data a tensor may become another one at the same address, or a gradient a shorter one: the table is made anew
+    then, where the layouts are checked, instead of being given other addresses."""
+    made = []
+    table = ops.AdamW._table
+
+    def counted(self, *args):
+        made.append(0)
+        return table(self, *args)
+    p = param(6, 6)
+    opt = ops.AdamW([p])
+    opt._table = counted.__get__(opt)
+    p.grad = torch.ones(6, 6)
+    opt.step()
+    p.grad = torch.ones(6, 6)                               # other storage alone is not that
+    held = torch.ones(64)                                   # (so that no address comes back)
+    opt.step()
+    assert len(made) == 1
+    p.grad.data = torch.ones(4)
+    opt.step()
+    assert len(made) == 2
+    p.grad.data = torch.ones(6, 6)
+    opt.step()
+    assert len(made) == 3
+    p.data = p.data.t()
+    opt.step()
+    assert len(made) == 4
+    del held
