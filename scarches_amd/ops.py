@@ -30,6 +30,7 @@ _F8_M, _F8_V = torch.float8_e4m3fn, torch.float8_e5m2
 # What a small call costs is its host side (a launch takes 4 us, each allocation 1.5): entry points are looked up once, the
 # device and the stream are asked for as numbers (current_stream() builds an object: 2 us).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device   # (tensors are there: initialised)
 _fns = {}
 
 
@@ -80,7 +81,7 @@ def _same_device(*tensors) -> int:
 
 def _call(index, name, *args):
     """One entry point of the library on device `index`, behind what its current stream holds."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = _fn(name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -543,7 +544,7 @@ class AdamW(torch.optim.Optimizer):
         scales = self.state_bits == 8
         for gi, group in enumerate(self.param_groups):
             # what the table was made of: addresses, sizes, types and layouts
-            key, grads, taken, bits, mask = [group["weight_decay"]], [], [], 0, 0
+            key, grads, taken, mask = [group["weight_decay"]], [], [], 0
             for p in group["params"]:
                 g = p.grad
                 mask <<= 1
@@ -553,19 +554,19 @@ class AdamW(torch.optim.Optimizer):
                 st = self.state[p]
                 if not st:
                     self._init_state(p)
-                at = g.data_ptr()
-                grads.append(at)
+                grads.append(g.data_ptr())
                 taken.append(p)
-                bits |= at
-                key += (p.data_ptr(), p.numel(), g.numel(), p.dtype, g.dtype,
-                        p.is_contiguous() and g.is_contiguous() or (p.stride(), g.stride()), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
+                key += (p.data_ptr(), p.numel(), p.dtype, g.nbytes, p.is_contiguous() and g.is_contiguous() or (p.stride(), g.stride()),
+                        st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
                 if scales:
                     key += (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr())
             if not grads:           # (nobody takes a step: nothing to count)
                 continue
             plan = self._plans.get(gi)
-            moved = plan is not None and plan["key"] == key and plan["grads"] != grads
-            if plan is None or plan["key"] != key or moved and (plan["captured"] or bits % 16):
+            known = plan is not None and plan["key"] == key
+            moved = known and plan["grads"] != grads
+            if not known or moved and (plan["captured"] or any(at % 16 for at in grads)
+                                       or any(p.grad.dtype != p.dtype for p in taken)):
                 plan = self._plans[gi] = self._table(gi, group, key, grads)
                 moved = False
             stream = _raw_stream(plan["index"])
@@ -597,7 +598,7 @@ class AdamW(torch.optim.Optimizer):
             if t is not None:       # (a call that raised has counted nothing)
                 self._host_steps[gi] = (t, mask)
             # the kernel writes through addresses: autograd has to hear that what it may have saved is not there any more
-            torch.autograd.graph.increment_version(taken)
+            torch._C._increment_version(taken)              # (torch.autograd.graph.increment_version)
         return loss
 
     # torch wraps step() to run its hooks and to be seen by the profiler, which takes 6 us: here only where one is wanted
