@@ -427,6 +427,7 @@ class AdamW(torch.optim.Optimizer):
         sd = super().state_dict()
         if self.state_bits == 8:
             sd["param_groups"] = [dict(group, seed=self.seed) for group in sd["param_groups"]]
+        sd["state"] = {pid: st for pid, st in sd["state"].items() if st}        # (looking one up leaves an empty one)
         for gi, packed in enumerate(sd["param_groups"]):
             if gi not in self._steps:
                 continue
@@ -453,7 +454,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("the state dict's lr and betas must be numbers")
         keys = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
         for st in state_dict["state"].values():
-            if set(st) - {"step"} != keys:
+            if set(st) - {"step"} not in (keys, set()):
                 raise ValueError(f"the state dict holds {sorted(st)}, this optimizer keeps {self.state_bits}-bit states")
         seeds = {int(group["seed"]) for group in state_dict["param_groups"] if "seed" in group}
         if len(seeds) > 1:
@@ -469,11 +470,13 @@ class AdamW(torch.optim.Optimizer):
             if not group["params"]:
                 continue
             for p, pid in zip(group["params"], packed["params"]):
-                st = state_dict["state"].get(pid)
-                steps.append(int(st.get("step", 0)) if st else 0)
-                if st:      # the types of the states are theirs, not the parameter's
+                st = state_dict["state"].get(pid, {})
+                steps.append(int(st.get("step", 0)))
+                if "exp_avg" in st:     # the types of the states are theirs, not the parameter's
                     self.state[p] = {k: st[k].to(p.device, torch.float32 if self.state_bits == 32 else st[k].dtype,
                                                  copy=True) for k in keys}
+                else:
+                    self.state.pop(p, None)
             self._group_steps(gi).copy_(torch.tensor(steps))
             if self._host_steps.get(gi, (0,))[0] is not None:
                 taken, mask = set(steps) - {0}, 0
@@ -583,7 +586,7 @@ class AdamW(torch.optim.Optimizer):
             if of is not None and of != mask:
                 t = None
             if torch.cuda.is_current_stream_capturing():    # replays read the table and what it points to
-                self._captured.append((plan, [(p, p.grad, dict(self.state[p])) for p in group["params"]]))
+                self._captured.append((plan, [(p, p.grad, dict(self.state[p])) for p in taken]))
                 plan["captured"] = True
                 if moved:   # the table changes when the graph runs, not now
                     del self._plans[gi]

@@ -149,3 +149,27 @@ def test_tensors_that_change_in_place(calls):
     opt.step()
     assert len(made) == 4
     del held
+
+
+def test_parameters_without_states(calls, monkeypatch):
+    """A parameter that never took a step has no entry in the state dict, also behind a capture or an error; dicts that hold an
+    empty one load."""
+    p, frozen = param(3), param(3)
+    opt = ops.AdamW([p, frozen])
+    p.grad = torch.ones(3)
+    opt.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    opt.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert set(opt.state_dict()["state"]) == {0}
+    opt.state[frozen]
+    sd = opt.state_dict()
+    assert set(sd["state"]) == {0}
+    sd["state"][1] = dict(step=0)
+    other = ops.AdamW([param(3), param(3)])
+    other.load_state_dict(sd)
+    assert set(other.state_dict()["state"]) == {0} and other._steps[0][1] == 0
+    joins = other.param_groups[0]["params"][1]
+    joins.grad = torch.ones(3)
+    other.step()
+    assert set(other.state[joins]) == {"exp_avg", "exp_avg_sq"}
