@@ -352,10 +352,10 @@ __global__ __launch_bounds__(256) void ln_bwd_long_kernel(const LnBwd a) {
 // dw and db from the slabs: 32 columns per workgroup, 32 threads a column, added in a fixed order.
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_dw_finish_kernel(const float* __restrict__ part, int slabs, int n,
-                                                            W* __restrict__ dw, W* __restrict__ db) {
+                                                            W* __restrict__ dw, W* __restrict__ db, long long first) {
     __shared__ float sum[32][33];
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const long long c = (long long)blockIdx.x * 32 + lane, width = 2LL * n;      // column of [dw | db]
+    const long long c = first + (long long)blockIdx.x * 32 + lane, width = 2LL * n;      // column of [dw | db]
     float v = 0.f;
     if (c < width) {
 #pragma unroll 8
@@ -502,9 +502,12 @@ int ln_bwd(LnBwd a, void* dw, void* db, hipStream_t st) {
         hipLaunchKernelGGL((ln_bwd_long_kernel<T, W>), dim3((unsigned)((n + 256LL * VEC - 1) / (256LL * VEC)), sh.slabs),
                            dim3(256), 0, st, a);
     }
-    if (dw || db)
-        hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((unsigned)((2LL * n + 31) / 32)), dim3(1024), 0, st, a.part,
-                           a.rows > 0 ? sh.slabs : 0, n, (W*)dw, (W*)db);
+    const long long columns = dw || db ? 2LL * n : 0;
+    for (long long c = 0; c < columns; c += 32 * MAX_BLOCKS) {           // (more than one launch from n = 2^24 on)
+        const long long left = (columns - c + 31) / 32;
+        hipLaunchKernelGGL((ln_dw_finish_kernel<W>), dim3((unsigned)(left < MAX_BLOCKS ? left : MAX_BLOCKS)), dim3(1024), 0, st,
+                           a.part, a.rows > 0 ? sh.slabs : 0, n, (W*)dw, (W*)db, c);
+    }
     SCA_CHECK_LAUNCH();
     return 0;
 }

@@ -1,0 +1,25 @@
+"""GPU tests of scarches_amd.ops at sizes that one launch does not hold (2^32 threads and more): widths, outputs and rows that
+the documentation allows.  References and bounds as in test_gpu_dense_ops."""
+import pytest
+import torch
+
+from tests.test_gpu_dense_ops import TYPES, gen, ln_check_bwd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from scarches_amd import ops as m
+    return m
+
+
+@pytest.mark.parametrize("n,dtype", [((1 << 24) + 5, t) for t in TYPES] + [((1 << 26) + 3, torch.float32)], ids=str)
+def test_layer_norm_gradients_of_wide_rows(ops, n, dtype):
+    x, dy = (torch.randn(2, n, device="cuda", generator=gen(s)).to(dtype) for s in (1, 2))
+    w = (1 + 0.2 * torch.randn(n, device="cuda", generator=gen(3))).to(dtype)
+    _, stats = ops.layer_norm_fwd(x, w, w)
+    ln_check_bwd(ops, dy, x, w, stats)
+    _, _, db = ops.layer_norm_bwd(dy, x, w, stats, (False, False, True))
+    assert torch.equal(db, (dy[0].float() + dy[1].float()).to(dtype))          # one rounding in fp32, one to the type
+    assert db[-1] != 0 and db[-1].isfinite()
