@@ -855,7 +855,8 @@ void quantize(const void* x, long long ldx, int dtype, long long rows, int k, in
     else if (dtype == SCA_BF16) quant_rows<sca_bf16>(x, ldx, rows, k, q, ldq, scale, al, st);
     else quant_rows<sca_f16>(x, ldx, rows, k, q, ldq, scale, al, st);
 }
-bool one_launch(long long M, int K) { return M <= QUANT_ROWS && K <= QUANT_K - 128; }
+// (N: the direct kernel takes 32 threads an output, and a launch fewer than 2^32)
+bool one_launch(long long M, int N, int K) { return M <= QUANT_ROWS && K <= QUANT_K - 128 && (N + 15LL) / 16 < 1 << 23; }
 // Pitch of the rows that sca_linear_i8 quantizes for itself.  Tiles want whole cache lines (128 x 128 tiles, 16384 x 256 x
 // 4000: 25.0 us, 28.8 with 16 bytes more); the direct kernel, whose 16 lanes read 16 rows, wants them to start in different
 // banks (16 x 4096 x 4000: 6.6 us on whole lines, 5.5 with an odd number of 16-byte pieces; 320 x 400 x 2000: 6.4, 5.2).
@@ -908,7 +909,7 @@ extern "C" int sca_gemm_i8(const int8_t* xq, long long ldx, const float* sx, con
 
 extern "C" long long sca_linear_i8_workspace_bytes(long long M, int N, int K) {
     if (M < 0 || N < 0 || N > MAX_N || K <= 0 || K > I8_MAX_K) return -1;
-    if (one_launch(M, K)) return 0;
+    if (one_launch(M, N, K)) return 0;
     return M * (pitch_of(K, takes_direct(M, N, K)) + 4) + (worth_aligning(M, N, K) ? N * pitch_of(K, false) : 0);
 }
 
@@ -922,7 +923,7 @@ extern "C" int sca_linear_i8(const void* x, long long ldx, int dtype, const int8
     if (!x || !wq || !sw || !y) return -1;
     hipStream_t st = (hipStream_t)stream;
     I8Args a{(const int8_t*)x, ldx, nullptr, wq, ldw, sw, bias, btype, y, ytype, ldy, M, N, K, 0, 0};
-    if (one_launch(M, K)) {
+    if (one_launch(M, N, K)) {
         if (dtype == SCA_F32) launch_direct<float>(a, st);
         else if (dtype == SCA_BF16) launch_direct<sca_bf16>(a, st);
         else launch_direct<sca_f16>(a, st);

@@ -23,3 +23,17 @@ def test_layer_norm_gradients_of_wide_rows(ops, n, dtype):
     _, _, db = ops.layer_norm_bwd(dy, x, w, stats, (False, False, True))
     assert torch.equal(db, (dy[0].float() + dy[1].float()).to(dtype))          # one rounding in fp32, one to the type
     assert db[-1] != 0 and db[-1].isfinite()
+
+
+@pytest.mark.parametrize("m", [1, 2, 3])
+def test_int8_linear_of_very_many_outputs(ops, m):
+    """Small integers: quantized without a remainder (the largest is 127), and sums that every type holds."""
+    n, k = (1 << 27) + 5, 4
+    x = torch.randint(-3, 4, (m, k), device="cuda", generator=gen(m)).float()
+    x[:, 0] = 127
+    wq = torch.randint(-3, 4, (n, k), device="cuda", generator=gen(4), dtype=torch.int8)
+    ws = torch.ones(n, device="cuda")
+    got = ops.int8_linear(x, wq, ws)
+    for r in range(m):
+        want = sum(x[r, c] * wq[:, c].float() for c in range(k))
+        assert torch.equal(got[r], want), r

@@ -189,3 +189,11 @@ def test_adamw_takes_up_torch_states():
     with pytest.raises(ValueError, match="8-bit states"):
         ops.AdamW([p], state_bits=8).load_state_dict(sd)
     assert opt.state_dict()["state"][0]["step"] == 2
+
+
+def test_one_launch_for_one_row_has_its_limit():
+    """A workspace (two launches) where the direct kernel would start 2^32 threads or more."""
+    lib = _lib.load()
+    most = (1 << 27) - 16
+    for m in (1, 2):
+        assert lib.sca_linear_i8_workspace_bytes(m, most, 8) == 0 and lib.sca_linear_i8_workspace_bytes(m, most + 1, 8) >= m * 12
