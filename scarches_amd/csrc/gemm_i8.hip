@@ -827,7 +827,7 @@ bool takes_direct(long long M, int N, int K) {
     if (tiles >= 1 << 23) return false;                                         // (fewer than 2^32 threads)
     return M <= 16 || tiles <= CUS || (tiles <= 5 * CUS / 2 && tiles * K <= 1200000);
 }
-void gemm_i8(const I8Args& a, hipStream_t st) {
+void gemm_i8_rows(const I8Args& a, hipStream_t st) {
     const bool aligned = !(((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.ldx | (uintptr_t)a.ldw) & 15);
     auto tiles = [&](int b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); };
     auto runs = [&](int b, int per_cu) { return (tiles(b) + per_cu * CUS - 1) / (per_cu * CUS); };
@@ -843,6 +843,20 @@ void gemm_i8(const I8Args& a, hipStream_t st) {
         if (runs(128, 2) * (4 + 0.0104 * a.K) < runs(64, 1) * (3.25 + 0.0028 * a.K))
             launch_tile<128, 128, 2, 2, 64, 4, 1, false>(a, st);
         else launch_tile<64, 64, 2, 2, 128, 2, 4, false>(a, st);
+    }
+}
+// Fewer than 2^32 threads a launch: rows beyond 2^23 tiles of 128 x 128 (256 threads; of the other tiles the rule above takes
+// fewer) in slices.
+void gemm_i8(const I8Args& a, hipStream_t st) {
+    const long long wide = (a.N + 127LL) / 128, most = (wide < 1 << 23 ? (1 << 23) / wide : 1) * 128;
+    const int size = a.ytype == SCA_F32 ? 4 : 2;
+    I8Args s = a;
+    for (long long m = 0; m < a.M; m += most) {
+        s.x = a.x + m * a.ldx;
+        s.sx = a.sx + m;
+        s.y = (char*)a.y + m * a.ldy * size;
+        s.M = a.M - m < most ? a.M - m : most;
+        gemm_i8_rows(s, st);
     }
 }
 

@@ -37,3 +37,18 @@ def test_int8_linear_of_very_many_outputs(ops, m):
     for r in range(m):
         want = sum(x[r, c] * wq[:, c].float() for c in range(k))
         assert torch.equal(got[r], want), r
+
+
+def test_int8_matmul_of_very_many_rows(ops):
+    """Rows behind the first slice of a launch's worth, with an odd pitch."""
+    m, n, k = (1 << 31) + 70, 1, 1
+    xq = torch.empty(m, k, dtype=torch.int8, device="cuda").random_(-3, 4, generator=gen(1))
+    sx = torch.ones(m, device="cuda")
+    sx[-5:] = 2.0
+    wq = torch.full((n, k), 3, dtype=torch.int8, device="cuda")
+    got = ops.int8_matmul(xq, sx, wq, torch.ones(n, device="cuda"), None, torch.bfloat16)
+    xq.mul_(3)                                              # (within int8)
+    xq[-5:].mul_(2)
+    step = 1 << 28
+    for lo in range(0, m, step):
+        assert torch.equal(got[lo:lo + step], xq[lo:lo + step].bfloat16()), lo
