@@ -903,8 +903,11 @@ extern "C" int sca_csr_quant_rows_i8(const int64_t* indptr, const int32_t* indic
     if (ldq > CSR_LDS) return -2;
     if (B == 0) return 0;
     if (!indptr || !indices || !data || !q || !scale) return -1;
-    hipLaunchKernelGGL(csr_quant_rows_kernel, dim3(B), dim3(64), ldq, (hipStream_t)stream, indptr, indices, data, row_ids,
-                       apply_log1p, q, ldq, scale);
+    constexpr int MOST = 1 << 25;                // (fewer than 2^32 threads a launch)
+    for (long long b = 0; b < B; b += MOST)
+        hipLaunchKernelGGL(csr_quant_rows_kernel, dim3((unsigned)(B - b < MOST ? B - b : MOST)), dim3(64), ldq,
+                           (hipStream_t)stream, row_ids ? indptr : indptr + b, indices, data, row_ids ? row_ids + b : nullptr,
+                           apply_log1p, q + b * ldq, ldq, scale + b);
     SCA_CHECK_LAUNCH();
     return 0;
 }

@@ -52,3 +52,23 @@ def test_int8_matmul_of_very_many_rows(ops):
     step = 1 << 28
     for lo in range(0, m, step):
         assert torch.equal(got[lo:lo + step], xq[lo:lo + step].bfloat16()), lo
+
+
+@pytest.mark.parametrize("chosen", [False, True])
+def test_csr_rows_of_very_many_cells(ops, chosen):
+    """Cells behind the first launch's, of all rows and of rows that are chosen (here: backwards)."""
+    from scarches_amd import _lib
+    lib, b = _lib.load(), (1 << 26) + 3
+    data = torch.empty(b, device="cuda").random_(0, 50, generator=gen(1))              # one count per cell, in column cell % 3
+    indptr = torch.arange(b + 1, device="cuda")
+    indices = (torch.arange(b, device="cuda") % 3).int()
+    rows = torch.arange(b - 1, -1, -1, device="cuda") if chosen else None
+    q = torch.full((b + 1, 16), 99, dtype=torch.int8, device="cuda")
+    scale = torch.full((b + 1,), -1.0, device="cuda")
+    _lib.check(lib.sca_csr_quant_rows_i8(indptr.data_ptr(), indices.data_ptr(), data.data_ptr(), _lib.ptr(rows), b, 3, 0, q.data_ptr(),
+                                         16, scale.data_ptr(), torch.cuda.current_stream().cuda_stream), "csr_quant")
+    if chosen:
+        data, indices = data.flip(0), indices.flip(0)
+    assert torch.equal(scale[:b], data / torch.full_like(data, 127)) and scale[b] == -1
+    want = (indices[:, None] == torch.arange(16, device="cuda", dtype=torch.int32)[None]) & (data > 0)[:, None]
+    assert torch.equal(q[:b], want.to(torch.int8) * 127) and (q[b] == 99).all()
