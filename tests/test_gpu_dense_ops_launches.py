@@ -1,9 +1,10 @@
 """GPU tests of scarches_amd.ops at sizes that one launch does not hold (2^32 threads and more): widths, outputs and rows that
 the documentation allows.  References and bounds as in test_gpu_dense_ops."""
+import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_dense_ops import TYPES, gen, ln_check_bwd
+from tests.test_gpu_dense_ops import TYPES, gen, grid_ref, ln_check_bwd, philox_words
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +73,31 @@ def test_csr_rows_of_very_many_cells(ops, chosen):
     assert torch.equal(scale[:b], data / torch.full_like(data, 127)) and scale[b] == -1
     want = (indices[:, None] == torch.arange(16, device="cuda", dtype=torch.int32)[None]) & (data > 0)[:, None]
     assert torch.equal(q[:b], want.to(torch.int8) * 127) and (q[b] == 99).all()
+
+
+def words_at(first, n, tensor, t, seed, monkeypatch):
+    """Random words of elements [first, first + n) of a tensor, first a multiple of 4: the counter starts there."""
+    arange = np.arange
+    monkeypatch.setattr(np, "arange", lambda k, dtype: arange(first // 4, first // 4 + k, dtype=dtype))
+    words = philox_words(n, tensor, t, seed)
+    monkeypatch.undo()
+    return words
+
+
+def test_adamw_8_bits_behind_32_bit_offsets(ops, monkeypatch):
+    """The codes of the last block of a tensor of more than 2^31 values, value by value."""
+    n, few = (1 << 31) + 1111, 1111 % 256
+    first = n - few
+    assert first % 256 == 0
+    x = torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16)
+    x.grad = torch.full((n,), 0.25, device="cuda", dtype=torch.bfloat16)
+    x.grad[first:] = torch.linspace(-2, 2, few, device="cuda").bfloat16()
+    opt = ops.AdamW([x], lr=0.1, state_bits=8, seed=3)
+    opt.step()
+    st, g = opt.state[x], x.grad[first:].double().cpu()
+    words = words_at(first, few, 0, 1, 3, monkeypatch)
+    for key, value, rnd, kind in (("exp_avg", (1 - 0.9) * g, words & 0xffff, torch.float8_e4m3fn),
+                                  ("exp_avg_sq", (1 - 0.999) * g * g, words >> 16, torch.float8_e5m2)):
+        code, scale = grid_ref(value.float().numpy(), rnd, kind)
+        np.testing.assert_array_equal(st[key][first:].view(torch.uint8).cpu().numpy(), code[:few])
+        assert st[key + "_scale"][-1].item() == scale[0] and len(set(code[:few])) > 20, key

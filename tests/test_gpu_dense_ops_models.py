@@ -219,3 +219,39 @@ def test_latent_from_csr_and_from_dense_rows(model, monkeypatch):
         two = m.get_latent(*args, mean=True, int8=True)
         exact = m.get_latent(*args, mean=True)
     assert np.array_equal(one, two) and np.isfinite(one).all() and not np.array_equal(one, exact)
+
+
+@pytest.mark.parametrize("decay", [0.0, 10.0])
+@pytest.mark.parametrize("model", ["trvae", "expimap", "scpoli"])
+def test_every_step_of_a_trainer_is_adamw(model, decay):
+    """Each step that a trainer takes, as it launches it by default, against the formula on the gradient that the step left."""
+    kw = dict(n_epochs=2, lr=1e-3, eps=0.02, batch_size=64, monitor=False, optimizer="adamw", weight_decay=decay)
+    with contextlib.redirect_stdout(io.StringIO()):
+        m = small_model(model)
+        if model == "expimap":
+            kw["alpha"] = 1e-4
+        if model == "scpoli":
+            kw["pretraining_epochs"] = 2
+        eng = m.model.engine()
+        name = "adam_step" if model == "scpoli" else "train_step"
+        step, taken = getattr(eng, name), []
+
+        def parts():
+            return [[flat[eng.offsets[k]:eng.offsets[k] + eng.p[k].numel()].view_as(eng.p[k]).double().clone() for k in eng.names]
+                    for flat in (eng.flat_p, eng.flat_m, eng.flat_v)]
+
+        def checked(*args, **kwargs):
+            before = parts()
+            out = step(*args, **kwargs)
+            over = kwargs.get("wd_overrides") or {}
+            for k, p, mo, v in zip(eng.names, *before):
+                if eng.trainable[k]:
+                    ref, _, _, bound = adamw_ref(p, mo, v, eng.g[k].double(), eng.adam_t, 1e-3, 0.02, over.get(k, decay))
+                    within(eng.p[k], ref, bound, (eng.adam_t, k))
+                else:
+                    assert torch.equal(eng.p[k].double(), p), k
+            taken.append(eng.adam_t)
+            return out
+        setattr(eng, name, checked)
+        m.train(**kw)
+    assert len(taken) >= 10 and taken == list(range(1, len(taken) + 1))
