@@ -10,12 +10,14 @@ Reference path reproduced (see the kernel files for line-level citations):
 """
 from __future__ import annotations
 
+import gc
 import math
 from collections import OrderedDict
 from typing import Dict, List, Optional
 
 import numpy as np
 import os
+import sys
 
 import torch
 
@@ -26,6 +28,11 @@ ALIGN = 64  # floats (256 B) - every tensor starts on its own 256-byte boundary 
 
 def _round_up(n, a):
     return (n + a - 1) // a * a
+
+
+# Recorded plans and HIP graphs of engines that were dropped while a stream was being captured: they are let go in front of the
+# next capture, when the device may be waited for.
+_DROPPED = []
 
 
 class _Layer:
@@ -477,11 +484,31 @@ class CVAEEngine:
         if getattr(self, "_plans", None):
             # a HIP graph must not be destroyed (nor its buffers freed) while its last replay is still running
             torch.cuda.synchronize(self.device)
+            self._plans.clear()
         self._plans = {}
         self._mid_cache = {}
         self._gg_cache = {}
         self._tail_cache = {}
         self._ws_gen = getattr(self, "_ws_gen", 0) + 1
+
+    def close(self):
+        """Waits for the device and lets go of the recorded plans and HIP graphs (a step that follows makes them anew)."""
+        self._invalidate()
+
+    def __del__(self):
+        # As in _invalidate: the last replay of a graph may still run, on buffers that go with the engine.  In the middle of a
+        # capture (the garbage collector, another engine's step) nothing may be waited for or destroyed.
+        plans = self.__dict__.get("_plans")
+        if not plans or sys.is_finalizing():
+            return
+        try:
+            if torch.cuda.is_current_stream_capturing():
+                _DROPPED.append((plans, self.__dict__.get("ws")))
+                return
+            torch.cuda.synchronize(self.device)
+        except RuntimeError:        # (a device that has failed: nothing runs there any more)
+            pass
+        plans.clear()
 
     def _ensure(self, B):
         if B <= self.Bcap:
@@ -2031,9 +2058,7 @@ class CVAEEngine:
     def _train_step_planned(self, row_ids, cond, B, alpha_kl, lr, eps, clip, weight_decay, world, use_graph,
                             wd_overrides, grad_weight, next_rows, plan_key, have_cur, do_next):
         pf_stage = (next_rows, self._rows_next, B) if do_next else None
-        key = plan_key()
-        plans = self._plans
-        g = plans.get(key)
+        g = self._plans.get(plan_key())
         fast = (g is not None and row_ids.dtype == torch.int64 and cond.dtype == torch.int32 and row_ids.is_cuda
                 and cond.is_cuda and row_ids.is_contiguous() and cond.is_contiguous()
                 and row_ids.numel() == B and cond.numel() == B)
@@ -2160,9 +2185,18 @@ class CVAEEngine:
             rows, cond, snap = self._warm(B, weight_decay, wd_overrides)
         torch.cuda.current_stream(self.device).wait_stream(s)
         out = dict(rows=rows, cond=cond)
+        if _DROPPED:
+            torch.cuda.synchronize(self.device)
+            _DROPPED.clear()
         gf = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(gf):
-            self._step_and_adam(rows, cond, B, weight_decay, wd_overrides, split)
+        collects = gc.isenabled()
+        gc.disable()            # (what it finds may hold graphs, events and pinned memory, which a capture must not see go)
+        try:
+            with torch.cuda.graph(gf):
+                self._step_and_adam(rows, cond, B, weight_decay, wd_overrides, split)
+        finally:
+            if collects:
+                gc.enable()
         out["fwd"] = gf
         self._restore(snap)
         return out

@@ -1,0 +1,95 @@
+"""What the engine does with its HIP graphs around a capture, and which launch mode "auto" takes (no GPU needed: the pieces are
+called on an engine without a device)."""
+import gc
+import types
+
+import pytest
+import torch
+
+from scarches_amd import engine as E
+
+
+@pytest.fixture
+def device(monkeypatch):
+    """A device that is never busy: what was asked of it, in order."""
+    log = types.SimpleNamespace(calls=[], capturing=False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: log.calls.append("synchronize"))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: log.capturing)
+    return log
+
+
+class Graph:
+    """Says when it is destroyed."""
+    def __init__(self, log):
+        self.log = log
+
+    def __del__(self):
+        self.log.calls.append("destroyed")
+
+
+def bare(log):
+    eng = E.CVAEEngine.__new__(E.CVAEEngine)
+    eng.device = "cuda:0"
+    eng._plans = {1: dict(fwd=Graph(log))} if log is not None else {}
+    return eng
+
+
+def test_graphs_go_behind_a_wait(device):
+    eng = bare(device)
+    eng._invalidate()
+    assert device.calls == ["synchronize", "destroyed"] and eng._plans == {}
+    eng = bare(device)
+    eng.close()
+    assert device.calls == ["synchronize", "destroyed"] * 2
+    del eng
+    assert device.calls == ["synchronize", "destroyed"] * 2         # nothing left to wait for
+    eng = bare(device)
+    del eng
+    assert device.calls == ["synchronize", "destroyed"] * 3
+
+
+def test_an_engine_that_goes_in_a_capture(device):
+    eng = bare(device)
+    eng.me = eng                                                    # (only the garbage collector finds it)
+    graph = eng._plans[1]["fwd"] = object()
+    device.calls.clear()
+    device.capturing = True
+    del eng
+    gc.collect()
+    assert device.calls == [] and len(E._DROPPED) == 1 and E._DROPPED[0][0][1]["fwd"] is graph
+    E._DROPPED.clear()
+
+
+def test_no_garbage_is_collected_in_a_capture(device, monkeypatch):
+    seen = []
+
+    class Capture:
+        def __init__(self, graph):
+            pass
+
+        def __enter__(self):
+            seen.append((gc.isenabled(), len(E._DROPPED)))
+
+        def __exit__(self, *exc):
+            return False
+    stream = types.SimpleNamespace(wait_stream=lambda s: None)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda **kw: stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: Capture(None))
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: "graph")
+    monkeypatch.setattr(torch.cuda, "graph", Capture)
+    eng = bare(None)
+    monkeypatch.setattr(eng, "_warm", lambda *a: (0, 0, 0), raising=False)
+    monkeypatch.setattr(eng, "_restore", lambda snap: None, raising=False)
+    E._DROPPED.append((dict(fwd=Graph(device)), None))
+
+    def step(*a):
+        seen.append(gc.isenabled())
+        if a[2] < 0:
+            raise RuntimeError("in the step")
+    monkeypatch.setattr(eng, "_step_and_adam", step, raising=False)
+    assert eng._capture(4, 0.0, None, False)["fwd"] == "graph"
+    assert seen[-2:] == [(False, 0), False] and gc.isenabled() and device.calls == ["synchronize", "destroyed"]
+    with pytest.raises(RuntimeError, match="in the step"):
+        eng._capture(-1, 0.0, None, False)
+    assert gc.isenabled()
