@@ -373,6 +373,7 @@ class CVAEEngine:
         self._pf_flags = (False, False) # (skip the gather at the head of the step, gather the next one at its end)
         self._rows_next = None
         self.overlap = True
+        self._graph_size = None         # cells of the step that is captured; 0: none is any more (_auto_launch)
         self._dp = None                 # set_dp(): rank / world / exact-MMD switch of data-parallel runs
         self._dp_ws = {}
         self._dp_n_global = None
@@ -1999,7 +2000,8 @@ class CVAEEngine:
                      "auto" for B > 8192 and for every data-parallel step (10240 cells: 0.757 ms against 0.784 as a
                      graph; the look-ahead loader below exists in this mode only);
           * True   : replayed as HIP graphs (one graph launch per step; best when launch-bound: 0.27 ms at B=128
-                     against 0.37 ms eager) - "auto" for B <= 8192 on one GPU.  Round 3 (300-step runs, plan / graph):
+                     against 0.37 ms eager) - "auto" for B <= 8192 on one GPU, for one batch size of an engine
+                     and up to its next encoder pass (_auto_launch).  Round 3 (300-step runs, plan / graph):
                      2048 cells 0.255 / 0.226 ms, 4096: 0.332 / 0.310, 6144: 0.438 / 0.426, 8192: 0.573 / 0.568 with
                      the MMD forked behind the output GEMM inside graphs (_fused_path); the plan is host-bound up to
                      ~5000 cells (0.25 - 0.33 ms of host time per step against 0.13 - 0.24 for a graph launch);
@@ -2014,7 +2016,7 @@ class CVAEEngine:
             # (world > 1: the gradient all-reduce is a host call between the two replayed halves of the step.  The
             # intermittent hangs of bench.py's two-rank one-GPU rehearsal came from ProcessGroupGloo's device-tensor
             # path, not from the launch mode: see distributed._host_staged.)
-            use_graph = True if (B <= GRAPH_MAX_B and world <= 1) else "plan"
+            use_graph = self._auto_launch(B, world)
         self._dp_world, self._dp_grad_weight = int(world), grad_weight
         if world > 1 and use_graph is True:
             use_graph = "plan"      # the all-reduce is a host call inside the recorded sequence (not graph-captured)
@@ -2054,6 +2056,15 @@ class CVAEEngine:
                                             wd_overrides, grad_weight, next_rows, plan_key, have_cur, do_next)
         finally:
             self._pf_flags = (False, False)
+
+    def _auto_launch(self, B, world):
+        """Launch mode of train_step("auto"): a HIP graph up to GRAPH_MAX_B cells on one GPU, else the recorded plan.
+
+        One batch size of an engine is captured, until an encoder pass runs between its steps: a captured step of 4096 cells
+        with a pass of encode() in between and a second capture for the ragged last minibatch once ended in a segmentation
+        fault inside the runtime's graph launch, and no cause was found.  So a ragged minibatch takes the plan, and so does
+        every step behind such a pass.  (use_graph=True captures whatever the engine did before.)"""
+        return True if B <= GRAPH_MAX_B and world <= 1 and self._graph_size in (None, B) else "plan"
 
     def _train_step_planned(self, row_ids, cond, B, alpha_kl, lr, eps, clip, weight_decay, world, use_graph,
                             wd_overrides, grad_weight, next_rows, plan_key, have_cur, do_next):
@@ -2198,6 +2209,8 @@ class CVAEEngine:
             if collects:
                 gc.enable()
         out["fwd"] = gf
+        if self._graph_size is None:
+            self._graph_size = B
         self._restore(snap)
         return out
 
@@ -2267,6 +2280,8 @@ class CVAEEngine:
         `int8` (quantize_first_layer()): the first layer's product, nearly all of the pass, in 8-bit integers."""
         L, P = self.lib, self.p
         self._pf = None         # ws["x"] is about to be overwritten
+        if self._graph_size is not None:
+            self._graph_size = 0
         self._ensure(B)
         eps = self._eps_or_zero(eps, B)
         ws = self.ws

@@ -17,18 +17,3 @@ def pytest_configure(config):
 @pytest.fixture(scope="session")
 def golden_dir():
     return GOLDEN
-
-
-# Cases whose process once ended in a fault that reading has not explained: off until a cause is shown (none is deleted).
-UNEXPLAINED = {
-    "test_gpu_look_ahead.py::test_ragged_last_minibatch_and_encode_between_steps":
-        "once ended in a segmentation fault of the host inside the runtime's graph launch (CUDAGraph.replay), after passing in "
-        "every earlier run of the suite; no cause found by reading, so it stays off",
-}
-
-
-def pytest_collection_modifyitems(items):
-    for item in items:
-        for name, reason in UNEXPLAINED.items():
-            if item.nodeid.endswith(name):
-                item.add_marker(pytest.mark.skip(reason=reason))

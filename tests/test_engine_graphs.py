@@ -29,7 +29,7 @@ class Graph:
 
 def bare(log):
     eng = E.CVAEEngine.__new__(E.CVAEEngine)
-    eng.device = "cuda:0"
+    eng.device, eng._graph_size = "cuda:0", None
     eng._plans = {1: dict(fwd=Graph(log))} if log is not None else {}
     return eng
 
@@ -93,3 +93,24 @@ def test_no_garbage_is_collected_in_a_capture(device, monkeypatch):
     with pytest.raises(RuntimeError, match="in the step"):
         eng._capture(-1, 0.0, None, False)
     assert gc.isenabled()
+
+
+def test_auto_captures_one_batch_size(device, monkeypatch):
+    """A ragged last minibatch, and everything behind an encoder pass, takes the recorded plan."""
+    eng = bare(None)
+    assert eng._auto_launch(4096, 1) is True and eng._auto_launch(E.GRAPH_MAX_B + 1, 1) == "plan" == eng._auto_launch(4096, 2)
+    eng._graph_size = 4096
+    assert eng._auto_launch(4096, 1) is True and eng._auto_launch(1000, 1) == "plan"
+
+    def stop(B):
+        raise KeyError("far enough")
+    for size, then in ((4096, 0), (None, None)):            # a pass in front of the first step changes nothing
+        eng._graph_size = size
+        monkeypatch.setattr(eng, "_ensure", stop, raising=False)
+        monkeypatch.setattr(eng, "lib", None, raising=False)
+        monkeypatch.setattr(eng, "p", None, raising=False)
+        with pytest.raises(KeyError):
+            eng.encode(None, None, 512)
+        assert eng._graph_size == then
+    eng._graph_size = 0
+    assert eng._auto_launch(4096, 1) == eng._auto_launch(128, 1) == "plan"
