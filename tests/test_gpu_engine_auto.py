@@ -1,0 +1,63 @@
+"""train_step("auto") over what ordinary training does: full minibatches as a HIP graph with ragged ones as the recorded plan
+between them, and the recorded plan alone behind an encoder pass.  The trajectory is that of the eager launches; bounds as in
+test_gpu_look_ahead."""
+import gc
+
+import pytest
+import torch
+
+from tests.test_gpu_look_ahead import assert_same, batches, data, make_engine, run        # noqa: F401 (data: a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def captured(eng):
+    return {k[0] for k in eng._plans if k[1]}
+
+
+def test_ragged_minibatches_between_captured_ones(data):            # noqa: F811
+    full, ragged = batches(data, 1024, 6, seed=11), batches(data, 300, 2, seed=12)
+    bs = full[:3] + ragged[:1] + full[3:] + ragged[1:]
+    ref = run(data, bs, False, ahead=False)
+    got = run(data, bs, "auto", ahead=True)
+    assert_same(got, ref)
+    assert captured(got[2]) == {1024} and {k[0] for k in got[2]._plans} == {1024, 300}
+
+
+def test_steps_behind_an_encoder_pass_are_planned(data):            # noqa: F811
+    """No captured step is replayed behind the pass, none is captured.  (A pass moves the counter of the random numbers, so the
+    eager run has the same ones.)"""
+    bs = batches(data, 1024, 4, seed=11)
+    probe = batches(data, 512, 1, seed=6)[0]
+    seen = []
+
+    def hook(eng, i, rows, cond, nxt):
+        if i in (0, 1):                                             # the one in front of the first step changes nothing
+            before = captured(eng)
+            eng.encode(probe[0], probe[1], 512)
+            if before:
+                seen.append(before)
+                for g in eng._plans.values():                       # (a replay would fail here, and not run)
+                    g["fwd"] = None
+        return rows, cond, nxt
+    ref = run(data, bs, False, ahead=False, hook=hook)
+    got = run(data, bs, "auto", ahead=True, hook=hook)
+    assert_same(got, ref)
+    assert seen == [{1024}] and any(not k[1] for k in got[2]._plans)
+
+
+def test_engines_that_go_while_their_step_runs(data):               # noqa: F811
+    """Dropped right behind an asynchronous step, and found by the collector: the device is idle afterwards, the next engine's
+    steps are its own."""
+    bs = batches(data, 1024, 3, seed=11)
+    ref = run(data, bs, False, ahead=False)
+    for cycle in (False, True):
+        eng = make_engine(data)
+        for rows, cond in bs:
+            eng.train_step(rows, cond, 1024, 0.5, 1e-3)
+        if cycle:
+            eng.me = eng
+        del eng
+        gc.collect()
+        assert torch.cuda.current_stream().query()
+        assert_same(run(data, bs, "auto", ahead=False), ref)
