@@ -769,7 +769,14 @@ void quant_rows(const void* x, long long ldx, long long rows, int k, int8_t* q, 
                 const AlignRows& al, hipStream_t st) {
     const int vecs = (k + vec_of<T>() - 1) / vec_of<T>();
 #define QUANT(TPR, V) return launch_quant<T, TPR, V>(x, ldx, rows, k, q, ldq, scale, al, st)
-    // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory.
+    // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory; many: a wave holds a row by
+    // itself and meets no barrier.  us of many / few threads a row, launches on the same rows (fp32; bf16 rows of twice the values
+    // alike):
+    //            64 rows     1000       2000       4000       8000       16000
+    //   n 1000   2.5 / 2.7   3.1 / 2.8  4.1 / 3.0  6.2 / 3.8  10.0 / 6.7  17.5 / 12.9
+    //   n 2000   2.6 / 3.0   3.2 / 3.4  4.3 / 3.9  7.0 / 6.8  13.5 / 13.2 23.7 / 24.5
+    //   n 4000   3.0 / 2.9   6.3 / 4.0  11.0 / 6.7 20.5 / 13.1 37.8 / 24.1 83.2 / 50.5
+    // (The two meet at some 700, 1500 and 100 rows there; bf16 rows of 4000 values near 4000 rows.  The bounds lie above that.)
     if (vecs <= 16) QUANT(16, 1);
     if (vecs <= 64) QUANT(64, 1);
     if (vecs <= 128) QUANT(64, 2);
@@ -808,18 +815,23 @@ void launch_direct(I8Args a, hipStream_t st) {
     hipLaunchKernelGGL((gemm_i8_direct_kernel<T>), dim3((unsigned)((long long)a.tiles_m * a.tiles_n)), dim3(512), 0, st, a);
 }
 
-// Which kernel: us of direct / 64 x 64 by four groups / 128 x 128 / 256 x 256 tiles, results in bf16 (M x N x K):
-//   1 x 4096 x 4000     4.9 / 9.2 / 17 / 43           512 x 512 x 2048      10.0 / 6.4 / 10.5 / 25
-//   16 x 8192 x 4000    10.2 / 11.0 / 18 / -          8192 x 128 x 2000     37 / 7.7 / 11.9 / 27
-//   128 x 128 x 2000    4.4 / 6.7 / 11.4 / 26         1024 x 1024 x 4096    59 / 10.3 / 20 / 43
-//   256 x 256 x 8000    9.8 / 14.3 / 27 / -           64 x 20000 x 128      15.5 / 8.7 / 5.3 / -
-//   320 x 400 x 2000    6.4 / 6.9 / 11.5 / -          2048 x 2048 x 2048    118 / 24 / 13.7 / 28
-//   300 x 300 x 4096    9.7 / 8.7 / 18 / 46           16384 x 256 x 4000    224 / 43 / 25 / 46
-//   509 x 282 x 1972    8.3 / 7.5 / 12.6 / 28         4096 x 4096 x 4096    - / 156 / 84 / 69
-//   1000 x 250 x 300    6.1 / 5.4 / 8.1 / -           65536 x 64 x 512      40 / 17 / 10.9 / 16.1
-// Direct: one workgroup per CU at most, or a few with short rows (or single cells, whose x is read from the caches); 64: no
-// more tiles than CUs.  Larger tiles read less; they need about one tile per CU, little of it lost behind the edges, and no
-// last run over the chip with few of them (21986 x 543 x 608, 258 tiles of 256: 38 us, 25 in tiles of 128).  Over 60 sizes
+// Which kernel: us of direct with x in whole cache lines, as int8_matmul gets it from quantize_int8 (with x as sca_linear_i8 lays
+// it out, pitch_of) / 64 x 64 by four groups / 128 x 128 / 256 x 256 tiles, results in bf16 (M x N x K):
+//   1 x 4096 x 4000      4.9 (4.9) / 9.0 / 17 / 42          512 x 512 x 2048       9.9 (7.4) / 6.4 / 10.6 / 25
+//   16 x 8192 x 4000    10.1 (8.0) / 10.9 / 18 / 43         300 x 300 x 4096       9.6 (7.2) / 8.7 / 18 / 46
+//   128 x 128 x 2000     4.4 (3.9) / 6.7 / 11.4 / 26        8192 x 128 x 2000     36 (27) / 7.6 / 11.8 / 27
+//   256 x 256 x 8000     9.8 (7.8) / 14.1 / 27 / 75         1024 x 1024 x 4096    58 (40) / 10.4 / 20 / 43
+//   320 x 400 x 2000     6.4 (5.3) / 6.9 / 11.5 / 26        64 x 20000 x 128      15.4 (15.3) / 8.6 / 5.3 / 7.5
+//   400 x 450 x 1500     7.2 (6.0) / 7.1 / 11.3 / 24        2048 x 2048 x 2048   116 (76) / 24 / 13.7 / 28
+//   1000 x 250 x 300     6.0 (5.9) / 5.4 / 8.0 / 14         16384 x 256 x 4000   225 (160) / 44 / 25 / 46
+//   4096 x 4096 x 4096   - / 153 / 83 / 67                  65536 x 64 x 512      39 (36) / 17 / 11.1 / 16.1
+// Direct: one workgroup per CU at most, or a few with short rows (or single cells, whose x is read from the caches).  640 tiles
+// and tiles * K = 1.2 million: over 264 sizes drawn with 257 to 1400 tiles and tiles * K from 0.15 to 6 million, x in whole lines,
+// that takes 1.2 % longer than the better of the two kernels, and no other bound of tiles * K is better (1 million: 1.3 %, 1.5
+// million: 1.4 %; direct / tile at up to 640 tiles: 0.75 up to 0.4 million, 0.88 to 1, 0.97 to 1.2, 1.06 to 2, 1.17 to 3).  x as
+// sca_linear_i8 lays it out suits the direct kernel further up (0.70, 0.74, 0.78, 0.83, 0.92): the same bound takes 6 % longer there.
+// 64: no more tiles than CUs.  Larger tiles read less; they need about one tile per CU, little of it lost behind the edges, and
+// no last run over the chip with few of them (21986 x 543 x 608, 258 tiles of 256: 37 us, 24.5 in tiles of 128).  Over 60 sizes
 // drawn between 2e9 and 1.3e11 products the rule takes 1 % longer than the best of the three.
 constexpr int CUS = 256;
 bool takes_direct(long long M, int N, int K) {

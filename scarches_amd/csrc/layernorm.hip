@@ -433,7 +433,14 @@ int ln_fwd(const void* x, long long ldx, long long rows, int n, const void* w, c
         const long long blocks = (rows + 63) / 64;
         FWD_MODE(4, 1, ROW_TINY);
     }
-    // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory.
+    // Few rows: a thread takes one or two vectors, so that the row is there after one trip to memory; many: a wave holds a row by
+    // itself and meets no barrier.  us of many / few threads a row, launches on the same rows:
+    //                 64 rows     1000       2000        4000        8000        16000
+    //   fp32 n 1000   2.6 / 2.9   3.5 / 3.5  4.6 / 4.3   7.3 / 6.2   12.3 / 10.7 21.9 / 20.8
+    //   fp32 n 2000   2.9 / 4.0   4.4 / 5.1  6.6 / 6.9   12.1 / 10.8 21.4 / 21.7 38.2 / 39.4
+    //   bf16 n 4000   3.3 / 5.4   5.3 / 6.6  7.9 / 8.9   13.3 / 13.1 22.5 / 24.9 41.0 / 41.9
+    //   fp32 n 4000   3.4 / 3.5   8.4 / 6.5  14.7 / 10.6 25.7 / 20.6 46.6 / 37.9 89.2 / 73.2
+    // (The two meet at some 1000, 3000, 4000 and 256 rows there; the bounds, 4096 and 1024, lie above that.)
     else if (vecs <= 4) FWD(4, 1);
     else if (vecs <= 16) FWD(16, 1);
     else if (vecs <= 32) FWD(32, 1);
