@@ -339,7 +339,8 @@ int sca_bn_bwd(const float* dh, int S, long long slab_stride, const float* extra
  * stats [2][rows] = (mean, rstd), fp32; may be NULL in the forward pass.  Sums and statistics are held in fp32, each
  * result is rounded once.  Outputs overlap no input.  sca_layernorm_bwd: dx, dw, db may
  * each be NULL; ws: scratch of sca_layernorm_bwd_workspace_floats(rows, n) floats (any contents on entry; not to be shared
- * by calls that may overlap), which may be NULL where neither dw nor db is asked for and n <= 16384.  Sums over rows are taken in a fixed order: the same call gives the same bits.
+ * by calls that may overlap), which may be NULL where neither dw nor db is asked for and n <= 16384.  Sums over rows are taken
+ * in a fixed order: the same call gives the same bits.
  * rows = 0: nothing is read, dw and db become 0.  -1 for an argument outside these ranges. */
 int sca_layernorm_fwd(const void* x, long long ldx, int dtype, long long rows, int n, const void* w, const void* b,
                       int wtype, float eps, void* y, long long ldy, float* stats, void* stream);
@@ -399,7 +400,8 @@ int sca_adamw_step(const sca_adamw_tensor* tensors, int n_tensors, const sca_ada
  * bias (may be NULL): btype 0 or ytype.  Any pitches and alignments; 16-byte aligned operands whose pitch is a multiple of
  * 16 take the faster loads.  The forward product y = x W^T of the reference's nn.Linear layers
  * (scarches/models/trvae/modules.py:21-27) for serving.
- * sca_linear_i8: both in one call, y = x W^T + bias with x of dtype quantized on the way; one or two rows take one launch.
+ * sca_linear_i8: both in one call, y = x W^T + bias with x of dtype quantized on the way; one or two rows take one launch
+ * (K <= 8064, N < 2^27).
  * ws: scratch of sca_linear_i8_workspace_bytes(M, N, K) bytes, 16-byte aligned (0 bytes: may be NULL), any contents on entry,
  * not to be shared by calls that may overlap. */
 int sca_gemm_i8_max_k(void);

@@ -336,8 +336,8 @@ class AdamW(torch.optim.Optimizer):
     state_bits=32: `exp_avg`, `exp_avg_sq` in float32 whatever the parameter's type.
     state_bits=8: `exp_avg` float8_e4m3fn and `exp_avg_sq` float8_e5m2, each with one float32 power of two per 256 elements
     (`exp_avg_scale`, `exp_avg_sq_scale`): 2.03 bytes per value instead of 8.  Rounding to 8 bits is stochastic, from a
-    generator of (seed, parameter, element, step): the same seed gives the same run, and a state dict holds it.  A gradient that is not finite makes
-    the moments of its 256 elements NaN.
+    generator of (seed, parameter, element, step): the same seed gives the same run, and a state dict holds it.  A gradient
+    that is not finite makes the moments of its 256 elements NaN.
 
     The step number of each parameter lies on the device, so `step()` may be captured into a HIP graph after one ordinary
     call (lr and the other scalars are taken as they are at capture; a graph captured before `load_state_dict` goes on with the
@@ -559,8 +559,8 @@ class AdamW(torch.optim.Optimizer):
                     self._init_state(p)
                 grads.append(g.data_ptr())
                 taken.append(p)
-                key += (p.data_ptr(), p.numel(), p.dtype, g.nbytes, p.is_contiguous() and g.is_contiguous() or (p.stride(), g.stride()),
-                        st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
+                flat = p.is_contiguous() and g.is_contiguous() or (p.stride(), g.stride())
+                key += (p.data_ptr(), p.numel(), p.dtype, g.nbytes, flat, st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr())
                 if scales:
                     key += (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr())
             if not grads:           # (nobody takes a step: nothing to count)

@@ -405,7 +405,7 @@ def test_mid_direct_family_matches_staged_family(Hx, Zx, Bx, mask, monkeypatch):
 
 def test_captured_step_with_side_streams_waiting_for_each_other(data, monkeypatch):
     """hipStreamEndCapture of this ROCm segfaults when two forked streams of one capture wait for each other in both
-    directions (scripts/dbg/capture_crash_repro.py).  SCA_OUT_DW_AFTER_MMD=1 makes the step contain exactly that (the
+    directions.  SCA_OUT_DW_AFTER_MMD=1 makes the step contain exactly that (the
     output layer's weight-gradient GEMM on the second side stream waits for the MMD on the first, the gradient tail on
     the first later waits for that GEMM): the engine routes the second direction through the origin stream while a
     graph is captured, and the captured step gives the trajectory of the plain one."""
