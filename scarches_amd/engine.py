@@ -30,8 +30,8 @@ def _round_up(n, a):
     return (n + a - 1) // a * a
 
 
-# Recorded plans and HIP graphs of engines that were dropped while a stream was being captured: they are let go in front of the
-# next capture, when the device may be waited for.
+# What engines held (graphs and the buffers that their last replay may still use) that were dropped while a stream was being
+# captured: let go in front of the next capture, when the device may be waited for.
 _DROPPED = []
 
 
@@ -504,7 +504,7 @@ class CVAEEngine:
             return
         try:
             if torch.cuda.is_current_stream_capturing():
-                _DROPPED.append((plans, self.__dict__.get("ws")))
+                _DROPPED.append(dict(self.__dict__))
                 return
             torch.cuda.synchronize(self.device)
         except RuntimeError:        # (a device that has failed: nothing runs there any more)

@@ -52,11 +52,13 @@ def test_an_engine_that_goes_in_a_capture(device):
     eng = bare(device)
     eng.me = eng                                                    # (only the garbage collector finds it)
     graph = eng._plans[1]["fwd"] = object()
+    buffer = eng.flat_p = object()
     device.calls.clear()
     device.capturing = True
     del eng
     gc.collect()
-    assert device.calls == [] and len(E._DROPPED) == 1 and E._DROPPED[0][0][1]["fwd"] is graph
+    assert device.calls == [] and len(E._DROPPED) == 1
+    assert E._DROPPED[0]["_plans"][1]["fwd"] is graph and E._DROPPED[0]["flat_p"] is buffer
     E._DROPPED.clear()
 
 
@@ -81,7 +83,7 @@ def test_no_garbage_is_collected_in_a_capture(device, monkeypatch):
     eng = bare(None)
     monkeypatch.setattr(eng, "_warm", lambda *a: (0, 0, 0), raising=False)
     monkeypatch.setattr(eng, "_restore", lambda snap: None, raising=False)
-    E._DROPPED.append((dict(fwd=Graph(device)), None))
+    E._DROPPED.append(dict(_plans={1: dict(fwd=Graph(device))}))
 
     def step(*a):
         seen.append(gc.isenabled())
