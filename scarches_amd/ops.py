@@ -494,6 +494,9 @@ class AdamW(torch.optim.Optimizer):
         chunk = lib.sca_adamw_chunk_elements()
         block = lib.sca_adamw_block_elements()
         steps = self._group_steps(gi)
+        if steps.numel() != len(group["params"]):
+            raise RuntimeError(f"AdamW.step(): parameter group {gi} had {steps.numel()} parameters when it was first used and has "
+                               f"{len(group['params'])} now; others join by add_param_group()")
         first = sum(len(g["params"]) for g in self.param_groups[:gi])
         dev, rows = steps.device, []
         for i, p in enumerate(group["params"]):

@@ -5,6 +5,9 @@ import torch
 from scarches_amd import ops
 
 
+TABLE = ops.AdamW._table
+
+
 @pytest.fixture
 def calls(monkeypatch):
     made = []
@@ -173,3 +176,18 @@ def test_parameters_without_states(calls, monkeypatch):
     joins.grad = torch.ones(3)
     other.step()
     assert set(other.state[joins]) == {"exp_avg", "exp_avg_sq"}
+
+
+def test_a_group_that_was_changed_by_hand(calls, monkeypatch):
+    """Each parameter's step number has its place in an array as long as the group was: no table over another length."""
+    monkeypatch.setattr(ops.AdamW, "_table", TABLE)
+    opt = ops.AdamW([param(3)])
+    opt.set_step(4)
+    for change in (lambda ps: ps.append(param(3)), lambda ps: ps.append(param(3)), lambda ps: ps.__delitem__(slice(None, None))):
+        change(opt.param_groups[0]["params"])
+        for p in opt.param_groups[0]["params"]:
+            p.grad = torch.ones(3)
+        if opt.param_groups[0]["params"]:
+            with pytest.raises(RuntimeError, match="add_param_group"):
+                opt.step()
+    assert not calls
