@@ -86,3 +86,23 @@ def test_transformations_are_refused(ops):
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             ops.layer_norm(forward_ad.make_dual(x, x), w.clone().requires_grad_(), w)
+
+
+def test_under_torch_compile(ops):
+    """A graph break: the operators run as ever, forward and backward."""
+    x, w = torch.randn(8, 40, device="cuda", generator=gen(1)), torch.ones(40, device="cuda", requires_grad=True)
+    wq, ws = ops.quantize_int8(torch.randn(5, 40, device="cuda", generator=gen(2)))
+
+    def f(v):
+        return ops.layer_norm(v * 2, w, w) + 1
+
+    def g(v):
+        return ops.int8_linear(v * 2, wq, ws) + 1
+    for backend in ("eager", "aot_eager"):
+        for call in (f, g):
+            torch._dynamo.reset()
+            assert torch.equal(torch.compile(call, backend=backend)(x), call(x)), (backend, call)
+        torch._dynamo.reset()
+        got, = torch.autograd.grad(torch.compile(f, backend=backend)(x).square().sum(), w)
+        want, = torch.autograd.grad(f(x).square().sum(), w)
+        assert torch.equal(got, want), backend
