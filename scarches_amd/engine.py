@@ -2001,7 +2001,7 @@ class CVAEEngine:
                      graph; the look-ahead loader below exists in this mode only);
           * True   : replayed as HIP graphs (one graph launch per step; best when launch-bound: 0.27 ms at B=128
                      against 0.37 ms eager) - "auto" for B <= 8192 on one GPU, for one batch size of an engine
-                     and up to its next encoder pass (_auto_launch).  Round 3 (300-step runs, plan / graph):
+                     and up to its next encoder pass (_auto_launch).  300-step runs, plan / graph:
                      2048 cells 0.255 / 0.226 ms, 4096: 0.332 / 0.310, 6144: 0.438 / 0.426, 8192: 0.573 / 0.568 with
                      the MMD forked behind the output GEMM inside graphs (_fused_path); the plan is host-bound up to
                      ~5000 cells (0.25 - 0.33 ms of host time per step against 0.13 - 0.24 for a graph launch);
@@ -2239,6 +2239,9 @@ class CVAEEngine:
     def quantize_first_layer(self):
         """(wq, scale) of the first encoder layer's weight for encode(int8=...): 8-bit integers with one scale per output."""
         from . import ops
+        genes, most = self.enc[0].n_in, self.lib._lib.sca_gemm_i8_max_k()
+        if genes > most:
+            raise ValueError(f"int8: cells of {genes} genes, the 8-bit product sums up to {most}")
         return ops.quantize_int8(self.p[self.enc[0].w])
 
     def _first_product(self, a, B, st, int8, max_split=None):

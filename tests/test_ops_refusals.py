@@ -197,3 +197,16 @@ def test_one_launch_for_one_row_has_its_limit():
     most = (1 << 27) - 16
     for m in (1, 2):
         assert lib.sca_linear_i8_workspace_bytes(m, most, 8) == 0 and lib.sca_linear_i8_workspace_bytes(m, most + 1, 8) >= m * 12
+
+
+def test_int8_latents_of_too_many_genes():
+    """Refused where the weight is quantized, before any cell is gathered."""
+    import types
+
+    from scarches_amd.engine import CVAEEngine
+    lib, layer = types.SimpleNamespace(_lib=_lib.load()), lambda n: [types.SimpleNamespace(n_in=n, w="w")]
+    most = _lib.load().sca_gemm_i8_max_k()
+    for n, error in ((most + 1, ValueError), (most, _lib.HipLibraryError)):
+        eng = types.SimpleNamespace(lib=lib, enc=layer(n), p=dict(w=t(2, n)))
+        with pytest.raises(error):
+            CVAEEngine.quantize_first_layer(eng)
