@@ -357,7 +357,7 @@ class CVAEEngine:
         self.step_ctr = torch.zeros(1, dtype=torch.int32, device=dev)      # mixed into the Philox streams
         self.losses = torch.zeros(4, dtype=torch.float32, device=dev)
         self.accum = torch.zeros(5, dtype=torch.float64, device=dev)
-        self.csr = None
+        self.csr = self._csr_at = None
         self.Bcap = 0
         # side stream: MMD runs beside the decoder, every dW / bias / condition-weight gradient beside the dX chain
         self.aux = torch.cuda.Stream(device=self.device, priority=int(os.environ.get("SCA_AUX_PRIO", "0")))
@@ -427,6 +427,7 @@ class CVAEEngine:
         assert indptr.dtype == torch.int64 and indices.dtype == torch.int32 and data.dtype == torch.float32
         assert indptr.device == self.device and indices.device == self.device and data.device == self.device
         self.csr = (indptr.contiguous(), indices.contiguous(), data.contiguous())
+        self._csr_at = tuple(t.data_ptr() for t in self.csr)        # (what recorded steps hold of it)
 
     def _masked_meta(self):
         """Tile-skipping plan of the masked decoder (csrc/masked_gemm.hip): genes in tiles of 32, per tile the sorted
@@ -2039,7 +2040,7 @@ class CVAEEngine:
                     tuple(sorted(k for k, v in self.trainable.items() if v)), self.use_mmd, self.mmd_on,
                     self.boundary, self.beta, torch.cuda.current_stream(self.device).cuda_stream,
                     self._dp_n_global if dp_exact else None, self.hsic_beta, self.dr_rate, self.seed, self.freeze,
-                    self.optimizer, self._ws_gen, self._pf_flags)
+                    self.optimizer, self._csr_at, self._ws_gen, self._pf_flags)
         self._ensure(B)
         # (launch plans only: captured into a HIP graph the trailing gather costs more than the head gather it
         #  replaces - 0.350 -> 0.360 ms at 4096 cells, 0.239 -> 0.245 ms at 1024)

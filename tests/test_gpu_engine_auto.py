@@ -61,3 +61,19 @@ def test_engines_that_go_while_their_step_runs(data):               # noqa: F811
         gc.collect()
         assert torch.cuda.current_stream().query()
         assert_same(run(data, bs, "auto", ahead=False), ref)
+
+
+@pytest.mark.parametrize("mode", ["plan", True, "auto"])
+def test_another_matrix_between_the_steps(data, mode):              # noqa: F811
+    """A recorded step holds the addresses of the matrix that it gathers from: cells of another one (a second data set, the
+    upload of a second trainer) are not to be read there."""
+    indptr, indices, vals = data["csr"]
+    other = (indptr, indices, (vals * 3 + 1).contiguous())
+    bs = batches(data, 1024, 6, seed=11)
+
+    def hook(eng, i, rows, cond, nxt):
+        if i in (2, 4):
+            eng.bind_csr(*(other if i == 2 else data["csr"]))
+        return rows, cond, None if i in (1, 3) else nxt
+    ref = run(data, bs, False, ahead=False, hook=hook)
+    assert_same(run(data, bs, mode, ahead=True, hook=hook), ref)
