@@ -419,6 +419,8 @@ class CVAEEngine:
             return eps
         z = getattr(self, "_zero_eps", None)
         if z is None or z.shape[0] < B:
+            if z is not None:
+                self._invalidate()
             z = self._zero_eps = torch.zeros(max(B, 1024), self.Zt, dtype=torch.float32, device=self.device)
         return z
 
@@ -2040,7 +2042,7 @@ class CVAEEngine:
                     tuple(sorted(k for k, v in self.trainable.items() if v)), self.use_mmd, self.mmd_on,
                     self.boundary, self.beta, torch.cuda.current_stream(self.device).cuda_stream,
                     self._dp_n_global if dp_exact else None, self.hsic_beta, self.dr_rate, self.seed, self.freeze,
-                    self.optimizer, self._csr_at, self._ws_gen, self._pf_flags)
+                    self.optimizer, self.noise_off, self._csr_at, self._ws_gen, self._pf_flags)
         self._ensure(B)
         # (launch plans only: captured into a HIP graph the trailing gather costs more than the head gather it
         #  replaces - 0.350 -> 0.360 ms at 4096 cells, 0.239 -> 0.245 ms at 1024)
