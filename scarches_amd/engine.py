@@ -2104,7 +2104,7 @@ class CVAEEngine:
             self._replay(g["fwd"])
         # what ws["x"] holds once this step's launches have run: the next minibatch, or nothing to rely on
         self._pf = (dict(rows=next_rows, ptr=next_rows.data_ptr(), version=next_rows._version, B=B, gen=self._ws_gen,
-                         csr=self.csr[0].data_ptr()) if do_next else None)
+                         csr=self._csr_at) if do_next else None)
         return self.losses
 
     def _pf_possible(self, next_rows, B):
@@ -2121,7 +2121,7 @@ class CVAEEngine:
         have been re-used by another tensor; in-place writes bump the shared version counter)."""
         pf = self._pf
         return (pf is not None and pf["B"] == B and pf["gen"] == self._ws_gen and self.csr is not None
-                and pf["csr"] == self.csr[0].data_ptr() and row_ids.dtype == torch.int64
+                and pf["csr"] == self._csr_at and row_ids.dtype == torch.int64
                 and row_ids.data_ptr() == pf["ptr"] and row_ids.numel() == B and row_ids.is_contiguous()
                 and row_ids._version == pf["version"] and pf["rows"]._version == pf["version"])
 
