@@ -106,3 +106,42 @@ def test_under_torch_compile(ops):
         got, = torch.autograd.grad(torch.compile(f, backend=backend)(x).square().sum(), w)
         want, = torch.autograd.grad(f(x).square().sum(), w)
         assert torch.equal(got, want), backend
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_training_step_in_one_graph(ops, bits):
+    """Forward, backward through autograd and the optimizer's step captured together, replayed between eager work, against the
+    same steps taken eagerly."""
+    def leaves():
+        return [t.requires_grad_() for t in (torch.randn(64, 96, device="cuda", generator=gen(1)), torch.ones(96, device="cuda"),
+                                             torch.zeros(96, device="cuda"))]
+
+    def step(ps, opt, dy):
+        opt.zero_grad(set_to_none=True)
+        ops.layer_norm(*ps).backward(dy)
+        opt.step()
+    a, b = leaves(), leaves()
+    oa, ob = (ops.AdamW(ps, lr=1e-2, state_bits=bits, seed=5) for ps in (a, b))
+    oa._host_steps[0] = (None, None)                        # (the device counts in both: the same bits)
+    static = torch.randn(64, 96, device="cuda", generator=gen(2))
+    for _ in range(3):
+        step(a, oa, static)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step(b, ob, static)
+    torch.cuda.current_stream().wait_stream(side)
+    ob.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(b, ob, static)
+    for i in range(6):
+        static.copy_(torch.randn(64, 96, device="cuda", generator=gen(10 + i)))
+        graph.replay()
+        step(a, oa, static)
+        if i % 2:
+            torch.cuda.synchronize()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q), i
+    assert ob.state_dict()["state"][2]["step"] == 9
