@@ -180,8 +180,8 @@ class HipLibraryError(RuntimeError):
 
 
 def build(verbose: bool = False) -> str:
-    """Compile the HIP sources in-tree for gfx950 (hipcc cross-compiles; no GPU needed)."""
-    res = subprocess.run(["make", "-C", CSRC, "-j8"], capture_output=True, text=True)
+    """Compile every HIP source in-tree for gfx950, also where a library is there (hipcc cross-compiles; no GPU needed)."""
+    res = subprocess.run(["make", "-B", "-C", CSRC, "-j8"], capture_output=True, text=True)
     if verbose:
         print(res.stdout[-2000:], res.stderr[-2000:])
     if res.returncode != 0 or not os.path.exists(LIB_PATH):
