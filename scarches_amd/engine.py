@@ -2188,7 +2188,7 @@ class CVAEEngine:
         finally:
             self._rec = None
             self._dp_dry = False
-        self._restore(snap)
+            self._restore(snap)
         return out
 
     def _capture(self, B, weight_decay, wd_overrides, split):
@@ -2211,10 +2211,10 @@ class CVAEEngine:
         finally:
             if collects:
                 gc.enable()
+            self._restore(snap)         # (what the warm-up changed, also where the capture failed)
         out["fwd"] = gf
         if self._graph_size is None:
             self._graph_size = B
-        self._restore(snap)
         return out
 
     def begin_step(self, alpha_kl, lr, eps=0.01, clip=0.0, stage=None, stage_next=None):

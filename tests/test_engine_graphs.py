@@ -82,7 +82,8 @@ def test_no_garbage_is_collected_in_a_capture(device, monkeypatch):
     monkeypatch.setattr(torch.cuda, "graph", Capture)
     eng = bare(None)
     monkeypatch.setattr(eng, "_warm", lambda *a: (0, 0, 0), raising=False)
-    monkeypatch.setattr(eng, "_restore", lambda snap: None, raising=False)
+    restored = []
+    monkeypatch.setattr(eng, "_restore", restored.append, raising=False)
     E._DROPPED.append(dict(_plans={1: dict(fwd=Graph(device))}))
 
     def step(*a):
@@ -94,7 +95,10 @@ def test_no_garbage_is_collected_in_a_capture(device, monkeypatch):
     assert seen[-2:] == [(False, 0), False] and gc.isenabled() and device.calls == ["synchronize", "destroyed"]
     with pytest.raises(RuntimeError, match="in the step"):
         eng._capture(-1, 0.0, None, False)
-    assert gc.isenabled()
+    assert gc.isenabled() and eng._graph_size == 4
+    with pytest.raises(RuntimeError, match="in the step"):
+        eng._record(-1, 0.0, None, False)
+    assert restored == [0, 0, 0] and eng._rec is None               # the warm-up's step is taken back, whatever came of it
 
 
 def test_auto_captures_one_batch_size(device, monkeypatch):
